@@ -208,6 +208,135 @@ int jv_qmatvec(int32_t type, const void* tiled, int32_t rows, int32_t cols, cons
 int jv_qmatvec_noalloc(int32_t type, const void* tiled, int32_t rows, int32_t cols, const float* x, float* y,
                        void* stream);
 
+/* ---- paged batches: many requests in one 8-bit KV cache, on device buffers -------------
+ * The operators a server runs for each step of many requests at once (no counterpart in the
+ * reference, whose KvCache holds one request in fp32). Like the QuantMatMul section they take
+ * device pointers and a cudaStream_t and return once the work is queued; they allocate nothing,
+ * so a step can be captured in a CUDA graph and replayed with other lengths. Each runs on the
+ * device that its buffers are on, whichever is current; `stream` must belong to that device.
+ * Calls that write the same cache pages, batch arrays or workspace must be ordered by the
+ * caller (one stream, or events): two graphs that share them must not run at the same time.
+ * What only the device knows (lengths, page ids, slots) is checked there: a bad value is not
+ * used but recorded in the two-word status (word 0 a JV_* status, the first one stays; word 1
+ * the site), which the caller zeroes once and reads when it likes.
+ *
+ * type is a GGML type id: 0 F32, 1 F16, 30 BF16. */
+
+#define JV_PAGE_TOKENS 64  /* tokens per page                                   */
+#define JV_SCALE_TOKENS 16 /* tokens that share a scale, per KV head and K or V */
+
+/* One layer of the cache. Page p holds int8 [kv_heads][2 (K, V)][64][128] at data + p * page_bytes
+ * (bytes; at least kv_heads * 16384, a multiple of 16) and fp32 [kv_heads][2][4], one scale for each
+ * 16 tokens, at scales + p * scale_stride (floats; at least kv_heads * 8, a multiple of 4): the value
+ * is int8 * scale. data and scales are 16-byte aligned. Layers may be interleaved inside a page
+ * through the strides. head_dim is 128. */
+typedef struct jv_kv8_cache {
+    void* data;
+    float* scales;
+    int64_t page_bytes, scale_stride;
+    int32_t pages, kv_heads;
+} jv_kv8_cache;
+
+/* A step of `requests` requests (1..4096) and the arrays jv_paged_plan writes for it. The bounds
+ * are the caller's; a step beyond one of them fails as a whole. group is the number of query heads
+ * per KV head (1..16). Rows of the token arrays behind the step's last token are left as they were. */
+typedef struct jv_paged_batch {
+    int32_t requests;
+    int32_t max_new;      /* most new tokens of one request                                */
+    int32_t max_tokens;   /* most new tokens of all requests: rows of the token arrays     */
+    int32_t max_blocks;   /* most pages of one request: columns of block_table             */
+    int64_t max_keys;     /* most tokens of all requests after the step                    */
+    int32_t group;        /* query heads per KV head                                       */
+    int32_t pages;        /* pages of the cache                                            */
+    int32_t* block_table; /* [requests][max_blocks] page of tokens 64 b .. 64 b + 63; in, out */
+    int32_t* lengths;     /* [requests] tokens after the step                              */
+    int32_t* starts;      /* [requests + 1] first new token of each request; the last: all */
+    int32_t* request_of;  /* [max_tokens]                                                  */
+    int32_t* positions;   /* [max_tokens]                                                  */
+    int64_t* slots;       /* [max_tokens] page * 64 + position % 64                        */
+    void* work;           /* jv_paged_work_bytes bytes, 16-byte aligned                    */
+    int32_t* status;      /* [2]                                                           */
+} jv_paged_batch;
+
+/* Bytes of jv_paged_batch.work for the batch's bounds; -1 and jv_last_error on a bad one. */
+int64_t jv_paged_work_bytes(const jv_paged_batch* batch);
+
+/* Block tables and slot maps from the requests' lengths. Request r holds cached[r] tokens, whose
+ * pages are in its row of block_table, and brings new_tokens[r] (0 allowed). The pages it lacks are
+ * taken from the end of free_pages[*n_free] (in request order, then block order: free_pages[*n_free
+ * - 1] first) and *n_free_out becomes the count left. Every array of the batch is written. cached may
+ * be lengths and n_free_out may be n_free, for a step that continues the last. Requests may share
+ * pages that are full; a page that a request writes to must be its own.
+ * If a bound of the batch is exceeded (JV_ERR_RANGE), free pages run out (JV_ERR_OOM) or a free page
+ * is not in the cache (JV_ERR_RANGE), no page is taken, lengths become cached and starts 0: the
+ * operators after it then do nothing. */
+int jv_paged_plan(const jv_paged_batch* batch, const int32_t* cached, const int32_t* new_tokens, const int32_t* free_pages,
+                  const int32_t* n_free, int32_t* n_free_out, void* stream);
+
+enum jv_rope_layout { JV_ROPE_ADJACENT = 0 /* pairs (2i, 2i + 1) */, JV_ROPE_HALF = 1 /* pairs (i, i + rotary_dim / 2) */ };
+enum jv_rope_scaling { JV_ROPE_PLAIN = 0, JV_ROPE_LINEAR = 1, JV_ROPE_YARN = 2 };
+
+/* Rotary positions (the rule of src/Jevstral/Model/Rope.cs:33-106, with angles in 64 bits, so that far
+ * positions keep theirs). turns[i] is pair i's frequency in turns per position; mscale multiplies every
+ * rotated element. temperature_scale and temperature_ctx are the query temperature of
+ * MinistralModel.cs:676-682 (off when either is 0): 1 + scale * ln(1 + floor(position / ctx)) on every
+ * element of heads that ask for it. jv_rope_init fills the struct; it is passed by value to the kernels. */
+typedef struct jv_rope_spec {
+    int32_t layout, rotary_dim;
+    float mscale, temperature_scale;
+    int32_t temperature_ctx, reserved;
+    double turns[128];
+} jv_rope_spec;
+
+/* rotary_dim: even, 2..256. factor > 0 (used by LINEAR and YARN), original_context, beta_fast and
+ * beta_slow (YARN). mscale is attn_factor, times 0.1 ln(factor) + 1 for YARN with factor > 1. */
+int jv_rope_init(jv_rope_spec* out, int32_t layout, int32_t rotary_dim, double base, int32_t scaling, double factor,
+                 int32_t original_context, double beta_fast, double beta_slow, double attn_factor);
+
+/* [tokens][heads][dim] in device memory, the last dimension contiguous; strides in elements. out may
+ * be NULL where only `in` is used, and may be `in` (with the same strides) for an operator in place;
+ * in and out must not overlap in any other way. */
+typedef struct jv_heads {
+    const void* in;
+    void* out;
+    int64_t in_token, in_head, out_token, out_head;
+    int32_t heads;
+    int32_t temperature; /* apply the spec's query temperature */
+} jv_heads;
+
+/* Rotates x[0..n) (queries and keys, n = 1 or 2) at positions[tokens]; the elements from rotary_dim on
+ * are copied. head_dim: even, up to 256, at least rotary_dim. tokens == 0 does nothing. */
+int jv_rope(const jv_rope_spec* spec, int32_t type, const int32_t* positions, int32_t tokens, int32_t head_dim,
+            const jv_heads* x, int32_t n, void* stream);
+
+/* Writes the batch's new keys and values (k->in and v->in, [tokens][kv_heads][128]) to their slots in 8
+ * bits. A block of 16 tokens has one scale per head for K and one for V: the largest magnitude written
+ * to it / 127. Where a block holds tokens of earlier steps the scale grows if it must, and their entries
+ * are rounded again at the new scale. With `rope` the keys are rotated first (rotary_dim a multiple of 8,
+ * at most 128) and, with q, the queries too: q->in of `type` to q->out of out_type. A value that is not
+ * finite is recorded as JV_ERR_NUMERIC; it is stored as 0 (not a number) or the block's largest value
+ * (an infinity) and does not count for the scale. Magnitudes below 2^-100 are stored as 0. */
+int jv_kv8_append(const jv_kv8_cache* cache, const jv_paged_batch* batch, int32_t type, const jv_heads* k,
+                  const jv_heads* v, const jv_rope_spec* rope, const jv_heads* q, int32_t out_type, void* stream);
+
+/* The values at slots[n] (page * 64 + row): k_out and v_out, [n][kv_heads][128] of `type`, rows
+ * `row_stride` elements apart. The rows of a negative slot are left as they were; a slot past the
+ * cache is recorded as JV_ERR_RANGE and its rows are left too. status may be NULL. */
+int jv_kv8_read(const jv_kv8_cache* cache, const int64_t* slots, int32_t n, int32_t type, void* k_out, void* v_out,
+                int64_t row_stride, int32_t* status, void* stream);
+
+/* Bytes of the workspace of jv_kv8_attention for the batch's bounds (nothing in it has to be
+ * initialised, and nothing is kept in it); -1 on a bad batch. */
+int64_t jv_kv8_attention_bytes(const jv_paged_batch* batch, int32_t kv_heads);
+
+/* Grouped-query attention of the batch's new tokens over the cache (their own keys appended before):
+ * q->in, [tokens][kv_heads * group][128] of `type` (F16 or BF16), to q->out of the same type. The token
+ * at position p sees keys p - window + 1 .. p, or 0 .. p when window is 0. A token without a visible key
+ * gives zeros. The result of a request depends on its own tokens only, bit for bit, not on what else is in
+ * the batch. Rows of q start on 16 bytes. */
+int jv_kv8_attention(const jv_kv8_cache* cache, const jv_paged_batch* batch, int32_t type, const jv_heads* q, float scale,
+                     int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- KV cache (src/Jevstral/Model/KvCache.cs) ----------------------------------------- */
 
 int32_t jv_kv_length(jv_ctx* ctx);                             /* KvCache.Length   :23     */

@@ -1,0 +1,98 @@
+// paged.h — what the paged-batch operators (paged.cu, kernels_rope.cu, kv8_attn.cu) share: the
+// layout of the 8-bit cache and of a plan's work lists, and the host-side checks.
+#pragma once
+
+#include "jv_internal.h"
+
+namespace jv {
+
+constexpr int PG_TOKENS = JV_PAGE_TOKENS;          // tokens per page
+constexpr int PG_BLOCK = JV_SCALE_TOKENS;          // tokens per scale
+constexpr int PG_DIM = 128;                        // head_dim
+constexpr int PG_PLANE = PG_TOKENS * PG_DIM;       // bytes of one K or V plane of a page
+constexpr int PG_MAX_REQUESTS = 4096;
+constexpr int PG_MAX_GROUP = 16;
+
+// A request whose new tokens x group give at most this many query rows is "small": its keys are
+// split into chunks that different CTAs take (kv8_attn.cu). The others go by tiles of query rows.
+constexpr int PG_SMALL_ROWS = 16;
+constexpr int PG_TILE_ROWS = 16;
+constexpr int PG_MAX_CHUNKS = 128;
+
+// Keys per chunk of a small request: 256, or as many more as keep the chunks at 128 at most.
+// It goes by the request's own length, so a request is cut alike in every batch.
+__host__ __device__ inline int pg_chunk_keys(int len) {
+    return 256 * ((len + 256 * PG_MAX_CHUNKS - 1) / (256 * PG_MAX_CHUNKS));
+}
+__host__ __device__ inline int pg_chunks(int len) {
+    return len <= 0 ? 0 : (len + pg_chunk_keys(len) - 1) / pg_chunk_keys(len);
+}
+
+// A plan's work lists, in jv_paged_batch.work.
+struct PlanView {
+    int32_t* head;      // [8]: small items, large items, append units
+    int32_t* first;     // [requests] first small item of each request
+    int32_t* prefix;    // [4][requests + 1]: needed pages, units, small items, large items before request r
+    int4* small_items;  // {request, chunk, chunks, 0}
+    int4* large_items;  // {request, tile, 0, 0}
+    int2* units;        // {request, block}: the 16-token blocks the step writes to
+    int64_t small_cap, large_cap, unit_cap, bytes;
+};
+PlanView plan_view(const jv_paged_batch& b);
+
+void check_batch(const jv_paged_batch* b, bool arrays);
+void check_cache(const jv_kv8_cache* c);
+void check_rows(const jv_heads* x, const char* name, int dim, int64_t tokens);
+int type_bytes(int type);  // 0 for a type the operators do not take
+
+// Runs on the device that `p` is on, for the guard's lifetime.
+struct OnDeviceOf {
+    int before = -1;
+    explicit OnDeviceOf(const void* p);
+    ~OnDeviceOf();
+    OnDeviceOf(const OnDeviceOf&) = delete;
+};
+
+template <class F>
+int paged_api(F&& f) {
+    try {
+        f();
+        return JV_OK;
+    } catch (const Error& e) {
+        return api_error(e.code, e.what());
+    } catch (const std::exception& e) {
+        return api_error(JV_ERR_ARG, e.what());
+    } catch (...) {
+        return api_error(JV_ERR_ARG, "an unknown error");
+    }
+}
+
+// Sites of the status word (word 1).
+enum PagedSite : int {
+    PS_PLAN_LENGTH = 96, PS_PLAN_TOKENS = 97, PS_PLAN_KEYS = 98, PS_PLAN_FREE = 99, PS_PLAN_PAGE = 100,
+    PS_APPEND_PAGE = 101, PS_APPEND_VALUE = 102, PS_READ_SLOT = 103, PS_READ_VALUE = 104, PS_ATTN_REQUEST = 105,
+    PS_ATTN_PAGE = 106, PS_ROPE_VALUE = 107
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void paged_report(int32_t* status, int code, int site) {
+    if (!status) return;
+    if (atomicCAS(status, 0, code) == 0) atomicExch(status + 1, site);
+}
+
+// The request's rows of a plan, as an operator after it uses them; false (and a report) where the
+// arrays do not hold what a plan writes.
+struct RequestRows {
+    int start, n_new, len;
+};
+__device__ __forceinline__ bool request_rows(const jv_paged_batch& b, int r, RequestRows& o) {
+    if (r < 0 || r >= b.requests) return false;
+    o.start = b.starts[r];
+    o.n_new = b.starts[r + 1] - o.start;
+    o.len = b.lengths[r];
+    return o.start >= 0 && o.n_new >= 0 && o.n_new <= b.max_new && o.start <= b.max_tokens - o.n_new && o.len >= 0 &&
+           o.len <= (int64_t)b.max_blocks * PG_TOKENS;
+}
+#endif
+
+}  // namespace jv

@@ -36,6 +36,27 @@ class JvLayout(C.Structure):
                 ("n_outputs", i32), ("end", i32), ("sparse", i32)]
 
 
+class JvKv8Cache(C.Structure):
+    _fields_ = [("data", vp), ("scales", vp), ("page_bytes", i64), ("scale_stride", i64), ("pages", i32), ("kv_heads", i32)]
+
+
+class JvPagedBatch(C.Structure):
+    _fields_ = [("requests", i32), ("max_new", i32), ("max_tokens", i32), ("max_blocks", i32), ("max_keys", i64),
+                ("group", i32), ("pages", i32)] + \
+               [(n, vp) for n in ("block_table", "lengths", "starts", "request_of", "positions", "slots", "work", "status")]
+
+
+class JvRopeSpec(C.Structure):
+    _fields_ = [("layout", i32), ("rotary_dim", i32), ("mscale", C.c_float), ("temperature_scale", C.c_float),
+                ("temperature_ctx", i32), ("reserved", i32), ("turns", C.c_double * 128)]
+
+
+class JvHeads(C.Structure):
+    # `in` is a Python keyword, so the input pointer is named src here
+    _fields_ = [("src", vp), ("out", vp), ("in_token", i64), ("in_head", i64), ("out_token", i64), ("out_head", i64),
+                ("heads", i32), ("temperature", i32)]
+
+
 SINK = C.CFUNCTYPE(None, C.c_void_p, C.c_char_p, f32p, i32, i32)
 
 # Every symbol include/jv.h declares, with its signature: (name, restype, argtypes).
@@ -67,6 +88,17 @@ SIGNATURES = [
     ("jv_qweight_pack", C.c_int, [i32, vp, i32, i32, vp, vp]),
     ("jv_qmatvec", C.c_int, [i32, vp, i32, i32, vp, vp, vp]),
     ("jv_qmatvec_noalloc", C.c_int, [i32, vp, i32, i32, vp, vp, vp]),
+    ("jv_paged_work_bytes", i64, [C.POINTER(JvPagedBatch)]),
+    ("jv_paged_plan", C.c_int, [C.POINTER(JvPagedBatch), vp, vp, vp, vp, vp, vp]),
+    ("jv_rope_init", C.c_int, [C.POINTER(JvRopeSpec), i32, i32, C.c_double, i32, C.c_double, i32, C.c_double, C.c_double,
+                               C.c_double]),
+    ("jv_rope", C.c_int, [C.POINTER(JvRopeSpec), i32, vp, i32, i32, C.POINTER(JvHeads), i32, vp]),
+    ("jv_kv8_append", C.c_int, [C.POINTER(JvKv8Cache), C.POINTER(JvPagedBatch), i32, C.POINTER(JvHeads),
+                                C.POINTER(JvHeads), C.POINTER(JvRopeSpec), C.POINTER(JvHeads), i32, vp]),
+    ("jv_kv8_read", C.c_int, [C.POINTER(JvKv8Cache), vp, i32, i32, vp, vp, i64, vp, vp]),
+    ("jv_kv8_attention_bytes", i64, [C.POINTER(JvPagedBatch), i32]),
+    ("jv_kv8_attention", C.c_int, [C.POINTER(JvKv8Cache), C.POINTER(JvPagedBatch), i32, C.POINTER(JvHeads), C.c_float,
+                                   i32, vp, i64, vp]),
     ("jv_kv_length", i32, [vp]),
     ("jv_kv_capacity", i32, [vp]),
     ("jv_kv_reset", C.c_int, [vp]),
