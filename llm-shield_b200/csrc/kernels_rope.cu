@@ -143,6 +143,76 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope(RopeKArgs a, int per_cta) {
     }
 }
 
+// The same with 16-byte accesses (V elements), for rows and pair halves that start on 16 bytes. A
+// "piece" is V consecutive elements: of adjacent pairs, or both halves of V half-split pairs, or V elements
+// behind rotary_dim. L lanes (a power of two) take a head's pieces.
+template <class T>
+union Vec {
+    uint4 raw;
+    T e[16 / sizeof(T)];
+};
+template <class T, int LAYOUT>
+__global__ void __launch_bounds__(RP_THREADS) k_rope_vec(RopeKArgs a, int per_cta, int lane_bits) {
+    constexpr int V = 16 / sizeof(T);
+    __shared__ __align__(16) float2 cs[RP_TOKENS][128];
+    __shared__ float temp[RP_TOKENS];
+    const int t0 = blockIdx.x * RP_TOKENS, nt = min(RP_TOKENS, a.tokens - t0);
+    const int half = a.spec.rotary_dim >> 1;
+    const int h0 = blockIdx.y * per_cta, nh = min(per_cta, a.n_heads - h0);
+    const int piece = threadIdx.x & ((1 << lane_bits) - 1), step = RP_THREADS >> lane_bits;
+    const int turned = LAYOUT == JV_ROPE_HALF ? half / V : 2 * half / V;  // pieces that are rotated
+    const int pieces = turned + (a.dim - 2 * half) / V;
+    const bool rotate = piece < turned;
+    const int e0 = rotate || LAYOUT == JV_ROPE_ADJACENT ? piece * V : 2 * half + (piece - turned) * V;
+    for (int i = threadIdx.x; i < nt * half; i += RP_THREADS) {
+        const int t = i / half, f = i % half;
+        cs[t][f] = rope_angle(a.spec.turns[f], a.positions[t0 + t], a.spec.mscale);
+    }
+    if (threadIdx.x < nt)
+        temp[threadIdx.x] = rope_temperature(a.positions[t0 + threadIdx.x], a.spec.temperature_ctx, a.spec.temperature_scale);
+    __syncthreads();
+    if (piece >= pieces) return;
+    int i = threadIdx.x >> lane_bits, t = i / nh, h = i % nh;
+    const int dt = step / nh, dh = step % nh;
+#pragma unroll 4
+    for (; t < nt;) {
+        const bool second = h0 + h >= a.x[0].heads;
+        const jv_heads& x = a.x[second ? 1 : 0];
+        const int hh = second ? h0 + h - a.x[0].heads : h0 + h;
+        const T* in = (const T*)x.in + (int64_t)(t0 + t) * x.in_token + (int64_t)hh * x.in_head + e0;
+        T* out = (T*)x.out + (int64_t)(t0 + t) * x.out_token + (int64_t)hh * x.out_head + e0;
+        const float k = x.temperature ? temp[t] : 1.f;
+        Vec<T> u, v;
+        u.raw = *(const uint4*)in;
+        if (LAYOUT == JV_ROPE_HALF && rotate) {
+            v.raw = *(const uint4*)(in + half);
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float2 c = cs[t][e0 + e];
+                const float p = ld1(u.e + e), q = ld1(v.e + e);
+                st1(u.e + e, __fsub_rn(__fmul_rn(p, c.x), __fmul_rn(q, c.y)) * k);
+                st1(v.e + e, __fadd_rn(__fmul_rn(p, c.y), __fmul_rn(q, c.x)) * k);
+            }
+            *(uint4*)(out + half) = v.raw;
+        } else if (LAYOUT == JV_ROPE_ADJACENT && rotate) {
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                const float2 c = cs[t][(e0 + e) >> 1];
+                const float p = ld1(u.e + e), q = ld1(u.e + e + 1);
+                st1(u.e + e, __fsub_rn(__fmul_rn(p, c.x), __fmul_rn(q, c.y)) * k);
+                st1(u.e + e + 1, __fadd_rn(__fmul_rn(p, c.y), __fmul_rn(q, c.x)) * k);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) st1(u.e + e, ld1(u.e + e) * k);
+        }
+        *(uint4*)out = u.raw;
+        t += dt;
+        h += dh;
+        if (h >= nh) h -= nh, t++;
+    }
+}
+
 // ------------------------------------------------------------ append
 
 struct AppendArgs {
@@ -321,12 +391,31 @@ bool vec4(const void* p, int64_t a, int64_t b, int elem) {
 }
 
 template <class T>
-void launch_rope(const RopeKArgs& a, cudaStream_t s) {
+void launch_rope(const RopeKArgs& a, int n, cudaStream_t s) {
     const int tiles = (a.tokens + RP_TOKENS - 1) / RP_TOKENS;
     // enough CTAs for the SMs when the tokens are few: the heads are split
-    const int split = std::max(1, std::min(a.n_heads, 296 / std::max(1, tiles)));
+    const int split = std::max(1, std::min(a.n_heads, 1184 / std::max(1, tiles)));
     const int per = (a.n_heads + split - 1) / split;
-    k_rope<T><<<dim3(tiles, (a.n_heads + per - 1) / per), RP_THREADS, 0, s>>>(a, per);
+    const dim3 grid(tiles, (a.n_heads + per - 1) / per);
+    constexpr int V = 16 / sizeof(T);
+    const bool half_split = a.spec.layout == JV_ROPE_HALF;
+    bool vec = a.dim % V == 0 && a.spec.rotary_dim % (half_split ? 2 * V : V) == 0;
+    for (int i = 0; i < n; i++) {
+        const jv_heads& x = a.x[i];
+        vec = vec && (uintptr_t)x.in % 16 == 0 && (uintptr_t)x.out % 16 == 0 && x.in_token % V == 0 && x.in_head % V == 0 &&
+              x.out_token % V == 0 && x.out_head % V == 0;
+    }
+    if (vec) {
+        const int pieces = (half_split ? a.dim - a.spec.rotary_dim / 2 : a.dim) / V;
+        int bits = 0;
+        while ((1 << bits) < pieces) bits++;
+        if (half_split)
+            k_rope_vec<T, JV_ROPE_HALF><<<grid, RP_THREADS, 0, s>>>(a, per, bits);
+        else
+            k_rope_vec<T, JV_ROPE_ADJACENT><<<grid, RP_THREADS, 0, s>>>(a, per, bits);
+    } else {
+        k_rope<T><<<grid, RP_THREADS, 0, s>>>(a, per);
+    }
     JV_CUDA(cudaGetLastError());
     note_launch();
 }
@@ -423,11 +512,11 @@ int jv_rope(const jv_rope_spec* spec, int32_t type, const int32_t* positions, in
         a.dim = head_dim;
         cudaStream_t s = (cudaStream_t)stream;
         if (type == T_F32)
-            launch_rope<float>(a, s);
+            launch_rope<float>(a, n, s);
         else if (type == T_F16)
-            launch_rope<__half>(a, s);
+            launch_rope<__half>(a, n, s);
         else
-            launch_rope<__nv_bfloat16>(a, s);
+            launch_rope<__nv_bfloat16>(a, n, s);
     });
 }
 

@@ -11,12 +11,15 @@
 // head of the group) on the 8-column side: S^T = K Q^T, O^T = V^T P^T. The order of the 128
 // dimensions inside a product is free, so a lane loads 16 consecutive int8 of its rows straight from
 // the cache into fragments; S^T becomes the operand P^T by one movmatrix per 8 x 8 block.
+#include <atomic>
 #include <cmath>
 #include <string>
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "paged.h"
+#include "tc_common.cuh"
 
 namespace jv {
 namespace {
@@ -43,6 +46,12 @@ __device__ __forceinline__ float ex2f(float x) {
     return y;
 }
 
+__device__ __forceinline__ float lg2f(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -61,12 +70,7 @@ __device__ __forceinline__ uint32_t pair_f16(uint32_t x, uint32_t sel) {
     return *(const uint32_t*)&h;
 }
 
-template <class T>
-__device__ __forceinline__ float2 unpack2(uint32_t x);
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t x) { return __half22float2(*(const __half2*)&x); }
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) {
+__device__ __forceinline__ float2 unpack_bf16(uint32_t x) {
     return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
 }
 template <class T>
@@ -80,6 +84,27 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *(const uint32_t*)&h;
+}
+
+// A row of 128 bf16 held by the four lanes of a group (16 pairs each), as fp16 times the power of two that is
+// returned: the one that puts the row's largest magnitude in [2^13, 2^14). Exact but for values 2^27 below it.
+__device__ __forceinline__ float q_to_f16(uint32_t (&q)[16]) {
+    float amax = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const float2 x = unpack_bf16(q[e]);
+        amax = fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y)));
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const int ex = min(max((int)((__float_as_uint(amax) >> 23) & 0xff), 14), 254);  // 2^(ex - 127) <= amax
+    const float up = __uint_as_float((uint32_t)(267 - ex) << 23);                     // 2^(13 - (ex - 127))
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const float2 x = unpack_bf16(q[e]);
+        q[e] = pack2<__half>(x.x * up, x.y * up);
+    }
+    return up;
 }
 
 // Rows [row0, row0 + 8 NT) of a request's query rows (row = new token * group + head of the group)
@@ -119,26 +144,7 @@ __device__ __forceinline__ void attend(const AttnKArgs& a, Smem<T, NT>& sm, cons
 #pragma unroll
             for (int e = 0; e < 16; e++) qf[n][e] = 0;
         }
-        if (std::is_same<T, __nv_bfloat16>::value) {
-            // bf16 -> fp16 times a power of two that puts the row's largest magnitude in [2^13, 2^14): exact
-            // but for values 2^27 below it
-            float amax = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const float2 x = unpack2<T>(qf[n][e]);
-                amax = fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y)));
-            }
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const int ex = min(max((int)((__float_as_uint(amax) >> 23) & 0xff), 14), 254);  // 2^(ex - 127) <= amax
-            const float up = __uint_as_float((uint32_t)(267 - ex) << 23);  // 2^(13 - (ex - 127))
-            f = 1.f / up;
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const float2 x = unpack2<T>(qf[n][e]);
-                qf[n][e] = pack2<__half>(x.x * up, x.y * up);
-            }
-        }
+        if (std::is_same<T, __nv_bfloat16>::value) f = 1.f / q_to_f16(qf[n]);
         f *= a.scale;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -290,86 +296,416 @@ __device__ __forceinline__ float4 joined(const Smem<T, NT>& sm, int r, int d4, f
 }
 
 template <class T>
-__device__ __forceinline__ void store_row(const AttnKArgs& a, const RequestRows& rr, int kvh, int row, int d4, float4 o, float l) {
+__device__ __forceinline__ void store_row(const AttnKArgs& a, int start, int kvh, int row, int d4, float4 o, float l) {
     const float inv = l == 0.f ? 0.f : 1.f / l;  // no visible key: zeros (a NaN stays one)
-    T* dst = (T*)a.q.out + (int64_t)(rr.start + row / a.b.group) * a.q.out_token +
+    T* dst = (T*)a.q.out + (int64_t)(start + row / a.b.group) * a.q.out_token +
              (int64_t)(kvh * a.b.group + row % a.b.group) * a.q.out_head + 4 * d4;
     *(uint2*)dst = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
 }
 
-// Small requests: persistent CTAs over (chunk of a request, KV head).
+// ------------------------------------------------------------ small requests
+
+// Small requests: persistent warps, each on its own, over (chunk of a request, row tile, KV head). A warp
+// streams its keys through two stages of 32 (K and V, one TMA tile each, stored with the 128-byte swizzle so
+// that the fragment loads below meet no bank twice); it refills a stage as soon as it has used it, with its
+// next keys or already with the first of its next item. Nothing joins the warps: a chunk's result goes to
+// the workspace (k_kv8_join), or out when the request has one chunk. Bound by HBM: 12 warps keep 96 KB per SM
+// in flight; a 16-key tile costs about 250 instructions, a third of the issue slots at the HBM rate.
+constexpr int KS_WARPS = 4;
+constexpr int KS_KEYS = 32;                        // keys per stage
+constexpr int KS_HALF = KS_KEYS * PG_DIM;          // bytes of K or V in a stage
+constexpr int KS_STAGES = 2;
+constexpr int KS_SMEM = KS_WARPS * KS_STAGES * 2 * KS_HALF + 1024;
+
+__device__ __forceinline__ void tma_keys(uint32_t dst, const CUtensorMap* map, int row, int kvh, int page, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
+            dst),
+        "l"(map), "r"(0), "r"(row), "r"(kvh), "r"(page), "r"(bar)
+        : "memory");
+}
+
+// One work item of a warp: its rows and keys; lane j holds page `page0 + j` of the request.
+struct KsItem {
+    int start, n_new, len, row0, n_rows, kvh, item, chunks, lo, hi, page0, pages;
+    bool valid;
+};
+
 template <class T, int NT>
-__global__ void __launch_bounds__(KA_THREADS) k_kv8_small(AttnKArgs a) {
-    __shared__ __align__(16) Smem<T, NT> sm;
-    const int kvh_n = a.c.kv_heads;
-    const int64_t n = (int64_t)min((int64_t)max(a.v.head[0], 0), a.v.small_cap) * kvh_n;
-    for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
-        const int item = (int)(w / kvh_n), kvh = (int)(w % kvh_n);
-        const int4 it = a.v.small_items[item];
-        RequestRows rr;
-        if (!request_rows(a.b, it.x, rr)) continue;
-        const int n_rows = rr.n_new * a.b.group;
-        if (n_rows > 8 * NT || n_rows > a.rows) continue;
-        const int ck = pg_chunk_keys(max(rr.len, 1));
-        int lo = it.y * ck, hi = min(rr.len, lo + ck);
-        if (a.window > 0) lo = max(lo, max(0, rr.len - rr.n_new + 1 - a.window));
-        attend<T, NT>(a, sm, rr, it.x, kvh, 0, lo, hi);
-        for (int e = threadIdx.x; e < n_rows * 32; e += KA_THREADS) {
-            const int r = e >> 5, d4 = e & 31;
-            float m, l;
-            const float4 o = joined<T, NT>(sm, r, d4, m, l);
-            if (it.z == 1) {
-                store_row<T>(a, rr, kvh, r, d4, o, l);
+__global__ void __launch_bounds__(KS_WARPS * 32, NT == 1 ? 3 : 2) k_kv8_small(AttnKArgs a, const __grid_constant__ CUtensorMap map) {
+    extern __shared__ uint8_t ks_raw[];
+    __shared__ uint64_t bars[KS_WARPS * KS_STAGES];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, i = lane & 3;
+    uint8_t* sm = ks_raw + ((1024u - (s_addr(ks_raw) & 1023u)) & 1023u) + warp * KS_STAGES * 2 * KS_HALF;
+    const uint32_t base = s_addr(sm), full = s_addr(bars + warp * KS_STAGES);
+    if (lane == 0) {
+        for (int s = 0; s < KS_STAGES; s++) mbar_init(full + 8 * s, 1);
+        fence_barrier_init();
+    }
+    __syncwarp();
+    pdl_wait();
+    pdl_launch_dependents();  // after the wait: what the plan wrote is then complete for the kernel after this one too
+    const int kvh_n = a.c.kv_heads, group = a.b.group;
+    const int64_t total = (int64_t)min((int64_t)max(a.v.head[0], 0), a.v.small_cap) * kvh_n;
+    const int64_t stride = (int64_t)gridDim.x * KS_WARPS;
+    int64_t unit = (int64_t)blockIdx.x * KS_WARPS + warp;
+
+    auto fetch = [&](int64_t u, int4& x, int4& y) {
+        if (u < total) {
+            x = a.v.small_items[2 * (u / kvh_n)];
+            y = a.v.small_items[2 * (u / kvh_n) + 1];
+        } else {
+            x = make_int4(-1, 0, 0, 0);
+            y = make_int4(0, 0, 0, 0);
+        }
+    };
+    auto decode = [&](int64_t u, int4 x, int4 y) {
+        KsItem t;
+        t.item = (int)(u / kvh_n), t.kvh = (int)(u % kvh_n);
+        t.start = y.x, t.n_new = y.y, t.len = y.z, t.chunks = x.z;
+        t.row0 = x.w * PG_ROW_TILE;
+        t.valid = x.x >= 0 && x.x < a.b.requests && rows_in_bounds(a.b, t.start, t.n_new, t.len) && t.row0 >= 0 &&
+                  t.row0 < t.n_new * group && x.y >= 0 && x.z >= 1;
+        if (!t.valid) t.n_new = t.len = t.row0 = 0;
+        t.n_rows = min(min(t.n_new * group - t.row0, a.rows), 8 * NT);
+        const int ck = pg_chunk_keys(t.len);
+        const int64_t from = (int64_t)x.y * ck;
+        t.lo = (int)min(from, (int64_t)t.len);
+        t.hi = (int)min(from + ck, (int64_t)t.len);
+        if (a.window > 0) t.lo = max(t.lo, t.len - t.n_new + t.row0 / group + 1 - a.window);
+        if (!t.valid || t.lo >= t.hi) t.lo = t.hi = 0;
+        t.page0 = t.lo / PG_TOKENS;
+        t.pages = t.page0 * PG_TOKENS + lane * PG_TOKENS < t.hi ? a.b.block_table[(int64_t)x.x * a.b.max_blocks + t.page0 + lane] : 0;
+        return t;
+    };
+    // Stage `n & 1` takes step t of an item (keys 32 t ..); a page that is not in the cache is not read.
+    auto issue = [&](const KsItem& it, int t, uint32_t n) {
+        const int page = __shfl_sync(0xffffffffu, it.pages, t * KS_KEYS / PG_TOKENS - it.page0);
+        const bool there = (unsigned)page < (unsigned)a.c.pages;
+        if (lane == 0) {
+            const uint32_t bar = full + 8 * (n & 1), dst = base + (n & 1) * 2 * KS_HALF;
+            mbar_expect_tx(bar, there ? 2 * KS_HALF : 0);
+            if (there) {
+                const int row = t * KS_KEYS % PG_TOKENS;
+                tma_keys(dst, &map, row, it.kvh, page, bar);
+                tma_keys(dst + KS_HALF, &map, PG_TOKENS + row, it.kvh, page, bar);
             } else {
-                const int64_t p = ((int64_t)item * kvh_n + kvh) * a.rows + r;
-                *(float4*)(a.part_o + p * PG_DIM + 4 * d4) = o;
-                if (d4 == 0) a.part_ml[p] = make_float2(m, l);
+                paged_report(a.b.status, JV_ERR_RANGE, PS_ATTN_PAGE);
             }
         }
-        __syncthreads();
+        __syncwarp();
+    };
+    auto scales_of = [&](const KsItem& it, int t, float2& k, float2& v) {
+        const int page = __shfl_sync(0xffffffffu, it.pages, t * KS_KEYS / PG_TOKENS - it.page0);
+        k = v = make_float2(1.f, 1.f);
+        if ((unsigned)page < (unsigned)a.c.pages) {
+            const float* p = a.c.scales + (int64_t)page * a.c.scale_stride + it.kvh * 8 + t * KS_KEYS % PG_TOKENS / PG_BLOCK;
+            k = *(const float2*)p;
+            v = *(const float2*)(p + 4);
+        }
+        return (unsigned)page < (unsigned)a.c.pages;
+    };
+
+    // Rows of a 16-key tile by fragment row: evens stay, odds are exchanged 4 apart, so that the lanes that load
+    // together (two fragment rows of K, four key pairs of V) find their 16-byte chunks in eight different places.
+    const int krow = (g & 1) ? ((g - 1) ^ 4) + 1 : g;
+    const int vrow = (2 * i ^ 4) + 1;
+    const uint32_t k_off = krow * PG_DIM, k_c0 = (i ^ (krow & 7)) << 4, k_c1 = ((4 + i) ^ (krow & 7)) << 4;
+    const uint32_t v_off0 = 2 * i * PG_DIM + ((g ^ (2 * i)) << 4), v_off1 = vrow * PG_DIM + ((g ^ vrow) << 4);
+
+    int4 px, py;
+    fetch(unit, px, py);
+    KsItem cur = decode(unit, px, py);
+    fetch(unit + stride, px, py);
+    uint32_t issued = 0, used = 0;  // stages over the warp's life
+    int at = cur.lo / KS_KEYS;      // next step of `cur` to issue
+    for (int s = 0; s < KS_STAGES && at * KS_KEYS < cur.hi; s++) issue(cur, at++, issued++);
+    for (; unit < total; unit += stride) {
+        const KsItem nxt = decode(unit + stride, px, py);
+        fetch(unit + 2 * stride, px, py);
+        int nat = nxt.lo / KS_KEYS;
+        if (cur.valid) {
+            uint32_t qf[NT][16];
+            float qs[NT][2], qb[NT][2], acc[NT][8][4], m[NT][2], l[NT][2];
+            int lo_key[NT][2], hi_key[NT][2];
+            const int first = cur.len - cur.n_new + cur.row0 / group;
+            const int last = cur.len - cur.n_new + (cur.row0 + cur.n_rows - 1) / group;
+            const int all_hi = min(first + 1, cur.hi), all_lo = max(cur.lo, a.window > 0 ? last + 1 - a.window : 0);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const int row = 8 * n + g;
+#pragma unroll
+                for (int e = 0; e < 16; e++) qf[n][e] = 0;
+                if (row < cur.n_rows) {
+                    const int r = cur.row0 + row;
+                    const T* src = (const T*)a.q.in + (int64_t)(cur.start + r / group) * a.q.in_token +
+                                   (int64_t)(cur.kvh * group + r % group) * a.q.in_head + 16 * i;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint4 x = *(const uint4*)(src + 64 * (j >> 1) + 8 * (j & 1));
+                        qf[n][4 * j] = x.x, qf[n][4 * j + 1] = x.y, qf[n][4 * j + 2] = x.z, qf[n][4 * j + 3] = x.w;
+                    }
+                }
+                float f = 1.f;
+                if (std::is_same<T, __nv_bfloat16>::value) f = 1.f / q_to_f16(qf[n]);
+                f *= a.scale;
+                // The K fragments are the bytes b + 128 as fp16 subnormals, (b + 128) 2^-24: an exact operand for
+                // one byte permute. q . kint = 2^24 (q . frag) - 128 sum q; the sum of the row is taken here.
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const float2 x = __half22float2(*(const __half2*)&qf[n][e]);
+                    sum += x.x + x.y;
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int col = 2 * i + e, r = 8 * n + col;
+                    qs[n][e] = __shfl_sync(0xffffffffu, f, 4 * col);
+                    qb[n][e] = -128.f * __shfl_sync(0xffffffffu, sum, 4 * col) * qs[n][e];
+                    qs[n][e] *= 16777216.f;
+                    const int pos = cur.len - cur.n_new + (cur.row0 + r) / group;
+                    hi_key[n][e] = r < cur.n_rows ? min(pos + 1, cur.hi) : 0;
+                    lo_key[n][e] = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+                    m[n][e] = -INFINITY;
+                    l[n][e] = 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[n][j][e] = 0.f;
+            }
+            float2 ks, vs;
+            bool there = false;
+            if (cur.lo < cur.hi) there = scales_of(cur, cur.lo / KS_KEYS, ks, vs);
+            for (int t = cur.lo / KS_KEYS; t * KS_KEYS < cur.hi; t++) {
+                const uint32_t st = used & 1;
+                if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, (used >> 1) & 1))) {
+                    if (lane == 0) paged_report(a.b.status, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_WAIT);
+                    if (issued - used > 1) mbar_wait(full + 8 * (st ^ 1), ((used + 1) >> 1) & 1);  // a copy still in flight
+                    return;
+                }
+                used++;
+                const float2 ks_t = ks;
+                float2 vs_t = vs;
+                const bool there_t = there;
+                if ((t + 1) * KS_KEYS < cur.hi) there = scales_of(cur, t + 1, ks, vs);
+                const int key0 = t * KS_KEYS;
+                if (there_t) {
+                    const uint8_t* kp = sm + st * 2 * KS_HALF;
+                    const bool second = key0 + PG_BLOCK < cur.hi;  // the second tile has a key of the request
+                    if (!(vs_t.x > 0.f)) vs_t.x = 1.f;  // a block of zeros
+                    if (!second || !(vs_t.y > 0.f)) vs_t.y = 1.f;
+                    float s[2][NT][4];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint4 kr[2][2];
+#pragma unroll
+                        for (int r = 0; r < 2; r++) {
+                            kr[r][0] = *(const uint4*)(kp + h * PG_BLOCK * PG_DIM + 8 * r * PG_DIM + k_off + k_c0);
+                            kr[r][1] = *(const uint4*)(kp + h * PG_BLOCK * PG_DIM + 8 * r * PG_DIM + k_off + k_c1);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) s[h][n][e] = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const uint32_t w0[4] = {kr[0][j].x, kr[0][j].y, kr[0][j].z, kr[0][j].w};
+                            const uint32_t w1[4] = {kr[1][j].x, kr[1][j].y, kr[1][j].z, kr[1][j].w};
+#pragma unroll
+                            for (int w = 0; w < 4; w++) {
+                                const uint32_t x0 = w0[w] ^ 0x80808080u, x1 = w1[w] ^ 0x80808080u;
+                                const uint32_t f[4] = {__byte_perm(x0, 0, 0x4140), __byte_perm(x1, 0, 0x4140), __byte_perm(x0, 0, 0x4342),
+                                                       __byte_perm(x1, 0, 0x4342)};
+#pragma unroll
+                                for (int n = 0; n < NT; n++) mma_f16(s[h][n], f, qf[n][8 * j + 2 * w], qf[n][8 * j + 2 * w + 1]);
+                            }
+                        }
+                    }
+                    const bool all = key0 >= all_lo && key0 + KS_KEYS <= all_hi;
+                    const float lv[2] = {lg2f(vs_t.x), lg2f(vs_t.y)}, iv[2] = {__frcp_rn(vs_t.x), __frcp_rn(vs_t.y)};
+                    const float kk[2] = {ks_t.x, ks_t.y};
+                    uint32_t pb[2][NT][2];
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        float e[2][4], mx[2];
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int c = 0; c < 2; c++) {
+                                const float ka = kk[h] * qs[n][c], kb = fmaf(kk[h], qb[n][c], lv[h]);
+                                e[h][c] = fmaf(s[h][n][c], ka, kb);
+                                e[h][c + 2] = fmaf(s[h][n][c + 2], ka, kb);
+                            }
+                        if (!all) {
+#pragma unroll
+                            for (int h = 0; h < 2; h++)
+#pragma unroll
+                                for (int x = 0; x < 4; x++) {
+                                    const int key = key0 + h * PG_BLOCK + krow + 8 * (x >> 1);
+                                    if (key >= hi_key[n][x & 1] || key < lo_key[n][x & 1]) e[h][x] = -INFINITY;
+                                }
+                        }
+                        bool move = false;
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            mx[c] = fmaxf(fmaxf(e[0][c], e[0][c + 2]), fmaxf(e[1][c], e[1][c + 2]));
+                            mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
+                            mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 8));
+                            mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 16));
+                            move |= mx[c] > m[n][c] + 8.f;
+                        }
+                        // the reference moves only when a score passes it by 2^8 (weights stay below 2^8)
+                        if (__any_sync(0xffffffffu, move)) {
+                            float alpha[2];
+#pragma unroll
+                            for (int c = 0; c < 2; c++) {
+                                const float mn = fmaxf(m[n][c], mx[c]);
+                                alpha[c] = m[n][c] == -INFINITY ? 0.f : ex2f(m[n][c] - mn);
+                                m[n][c] = mn;
+                                l[n][c] *= alpha[c];
+                            }
+#pragma unroll
+                            for (int j = 0; j < 8; j++)
+#pragma unroll
+                                for (int x = 0; x < 4; x++) acc[n][j][x] *= alpha[x & 1];
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+#pragma unroll
+                            for (int c = 0; c < 2; c++) {
+                                const float ref = m[n][c] == -INFINITY ? 0.f : m[n][c];
+                                e[h][c] = ex2f(e[h][c] - ref);
+                                e[h][c + 2] = ex2f(e[h][c + 2] - ref);
+                                l[n][c] = fmaf(e[h][c] + e[h][c + 2], iv[h], l[n][c]);
+                            }
+                            pb[h][n][0] = movmatrix_trans(pack2<__half>(e[h][0], e[h][1]));
+                            pb[h][n][1] = movmatrix_trans(pack2<__half>(e[h][2], e[h][3]));
+                        }
+                    }
+                    // O^T += V^T P^T: dimension 16 g + 2 j is the tile's row g, 16 g + 2 j + 1 its row g + 8. The V
+                    // fragments are signed integers (1024 + b + 128 - 1152): sums over thousands of keys would lose
+                    // what an offset left in them.
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint8_t* vp = kp + KS_HALF + h * PG_BLOCK * PG_DIM;
+                        const uint4 ra = *(const uint4*)(vp + v_off0), rb = *(const uint4*)(vp + v_off1);
+                        const uint4 rc = *(const uint4*)(vp + v_off0 + 8 * PG_DIM), rd = *(const uint4*)(vp + v_off1 + 8 * PG_DIM);
+                        const uint32_t va[4] = {ra.x, ra.y, ra.z, ra.w}, vb[4] = {rb.x, rb.y, rb.z, rb.w};
+                        const uint32_t vc[4] = {rc.x, rc.y, rc.z, rc.w}, vd[4] = {rd.x, rd.y, rd.z, rd.w};
+#pragma unroll
+                        for (int w = 0; w < 4; w++)
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                const uint32_t sel = u ? 0x7362 : 0x5140;
+                                const uint32_t lo = __byte_perm(va[w], vb[w], sel) ^ 0x80808080u;
+                                const uint32_t hi = __byte_perm(vc[w], vd[w], sel) ^ 0x80808080u;
+                                const uint32_t f[4] = {pair_f16(lo, 0x4140), pair_f16(lo, 0x4342), pair_f16(hi, 0x4140), pair_f16(hi, 0x4342)};
+#pragma unroll
+                                for (int n = 0; n < NT; n++) mma_f16(acc[n][2 * w + u], f, pb[h][n][0], pb[h][n][1]);
+                            }
+                    }
+                }
+                __syncwarp();
+                if (at * KS_KEYS < cur.hi)
+                    issue(cur, at++, issued++);
+                else if (nat * KS_KEYS < nxt.hi)
+                    issue(nxt, nat++, issued++);
+            }
+            // the chunk's result: lane (g, i) holds dimensions 16 g .. + 15 of rows 2 i and 2 i + 1
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    float x = l[n][c];
+                    x += __shfl_xor_sync(0xffffffffu, x, 4);
+                    x += __shfl_xor_sync(0xffffffffu, x, 8);
+                    x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    const int row = 8 * n + 2 * i + c;
+                    if (row >= cur.n_rows) continue;
+                    if (cur.chunks == 1) {
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2)
+                            store_row<T>(a, cur.start, cur.kvh, cur.row0 + row, 4 * g + j / 2,
+                                         make_float4(acc[n][j][c], acc[n][j][c + 2], acc[n][j + 1][c], acc[n][j + 1][c + 2]), x);
+                    } else {
+                        const int64_t p = ((int64_t)cur.item * kvh_n + cur.kvh) * a.rows + row;
+                        float4* dst = (float4*)(a.part_o + p * PG_DIM + 16 * g);
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2)
+                            dst[j / 2] = make_float4(acc[n][j][c], acc[n][j][c + 2], acc[n][j + 1][c], acc[n][j + 1][c + 2]);
+                        if (g == 0) a.part_ml[p] = make_float2(m[n][c], x);
+                    }
+                }
+        }
+        // what the next item still lacks of its first two stages (all of them after an item without keys)
+        cur = nxt;
+        at = nat;
+        while (issued - used < KS_STAGES && at * KS_KEYS < cur.hi) issue(cur, at++, issued++);
     }
 }
 
-// Joins the chunks of small requests: one CTA per (request, KV head, row), its warps over the chunks.
+// Joins the chunks of small requests: one CTA per (row, request, KV head), its warps over the chunks with a
+// running reference each, four chunks' loads in flight.
+constexpr int KJ_WARPS = 4;
 template <class T>
-__global__ void __launch_bounds__(256) k_kv8_join(AttnKArgs a) {
-    __shared__ float4 so[8][32];
-    __shared__ float sl[8];
-    const int request = blockIdx.x, kvh = blockIdx.y, row = blockIdx.z;
+__global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
+    __shared__ float4 so[KJ_WARPS][32];
+    __shared__ float2 sl[KJ_WARPS];
+    pdl_wait();
+    const int row = blockIdx.x, request = blockIdx.y, kvh = blockIdx.z;
     RequestRows rr;
     if (!request_rows(a.b, request, rr)) return;
     const int n_rows = rr.n_new * a.b.group, chunks = pg_chunks(rr.len);
     if (n_rows > PG_SMALL_ROWS || row >= n_rows || chunks < 2) return;
-    const int first = a.v.first[request];
-    if (first < 0 || first + chunks > a.v.small_cap) return;
+    const int first = a.v.first[request], item0 = first + row / PG_ROW_TILE * chunks;
+    if (first < 0 || item0 + chunks > a.v.small_cap) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t p0 = ((int64_t)first * a.c.kv_heads + kvh) * a.rows + row, step = (int64_t)a.c.kv_heads * a.rows;
-    float m = -INFINITY;
-    for (int c = lane; c < chunks; c += 32) m = fmaxf(m, a.part_ml[p0 + c * step].x);
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float ref = m == -INFINITY ? 0.f : m;
+    const int64_t p0 = ((int64_t)item0 * a.c.kv_heads + kvh) * a.rows + row % PG_ROW_TILE, step = (int64_t)a.c.kv_heads * a.rows;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-#pragma unroll 4
-    for (int c = warp; c < chunks; c += 8) {
-        const float2 ml = a.part_ml[p0 + c * step];
-        const float4 x = *(const float4*)(a.part_o + (p0 + c * step) * PG_DIM + 4 * lane);
-        const float f = ex2f(ml.x - ref);
-        l = fmaf(ml.y, f, l);
-        o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+    float m = -INFINITY, l = 0.f;
+    for (int c0 = warp; c0 < chunks; c0 += 4 * KJ_WARPS) {
+        float2 ml[4];
+        float4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int c = c0 + k * KJ_WARPS;
+            const bool in = c < chunks;
+            ml[k] = in ? a.part_ml[p0 + c * step] : make_float2(-INFINITY, 0.f);
+            x[k] = in ? *(const float4*)(a.part_o + (p0 + c * step) * PG_DIM + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        const float mn = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+        const float ref = mn == -INFINITY ? 0.f : mn, f0 = ex2f(m - ref);
+        m = mn;
+        l *= f0;
+        o.x *= f0, o.y *= f0, o.z *= f0, o.w *= f0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float f = ex2f(ml[k].x - ref);
+            l = fmaf(ml[k].y, f, l);
+            o.x = fmaf(x[k].x, f, o.x), o.y = fmaf(x[k].y, f, o.y), o.z = fmaf(x[k].z, f, o.z), o.w = fmaf(x[k].w, f, o.w);
+        }
     }
     so[warp][lane] = o;
-    if (lane == 0) sl[warp] = l;
+    if (lane == 0) sl[warp] = make_float2(m, l);
     __syncthreads();
     if (warp) return;
+    m = -INFINITY;
 #pragma unroll
-    for (int w = 1; w < 8; w++) {
+    for (int w = 0; w < KJ_WARPS; w++) m = fmaxf(m, sl[w].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < KJ_WARPS; w++) {
+        const float f = ex2f(sl[w].x - ref);
         const float4 x = so[w][lane];
-        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
-        l += sl[w];
+        l = fmaf(sl[w].y, f, l);
+        o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
     }
-    store_row<T>(a, rr, kvh, row, lane, o, l);
+    store_row<T>(a, rr.start, kvh, row, lane, o, l);
 }
 
 // Large requests: one CTA per (tile of 16 query rows, KV head), over all its keys.
@@ -391,20 +727,62 @@ __global__ void __launch_bounds__(KA_THREADS) k_kv8_large(AttnKArgs a) {
         for (int e = threadIdx.x; e < rows * 32; e += KA_THREADS) {
             float m, l;
             const float4 o = joined<T, 2>(sm, e >> 5, e & 31, m, l);
-            store_row<T>(a, rr, kvh, row0 + (e >> 5), e & 31, o, l);
+            store_row<T>(a, rr.start, kvh, row0 + (e >> 5), e & 31, o, l);
         }
         __syncthreads();
     }
 }
 
+// Query rows of a small item, and row tiles of a small request, at most.
+int tile_rows(const jv_paged_batch& b) { return (int)std::min<int64_t>(PG_ROW_TILE, (int64_t)b.max_new * b.group); }
 int small_rows(const jv_paged_batch& b) { return (int)std::min<int64_t>(PG_SMALL_ROWS, (int64_t)b.max_new * b.group); }
 
 struct Workspace {
     int64_t o, ml, bytes;
 };
 Workspace workspace(const jv_paged_batch& b, int kv_heads) {
-    const int64_t n = (b.requests + b.max_keys / 256) * kv_heads * small_rows(b);
+    const int64_t n = plan_view(b).small_cap * kv_heads * tile_rows(b);
     return {0, n * PG_DIM * 4, n * (PG_DIM * 4 + 8)};
+}
+
+// The cache as a 4-dimensional tensor of bytes, [page][kv head][K rows, V rows][128]; a box is the K or
+// the V of 32 tokens of one head. The encoder is looked up once through the runtime, so the library needs no link to libcuda.
+CUtensorMap page_map(const jv_kv8_cache& c) {
+    using Encode = decltype(&cuTensorMapEncodeTiled);
+    static const Encode encode = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        JV_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r));
+        if (!p || r != cudaDriverEntryPointSuccess) throw Error(JV_ERR_DEVICE, "the driver has no cuTensorMapEncodeTiled");
+        return (Encode)p;
+    }();
+    CUtensorMap m;
+    const cuuint64_t dims[4] = {PG_DIM, 2 * PG_TOKENS, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
+    const cuuint64_t strides[3] = {PG_DIM, 2 * PG_PLANE, (cuuint64_t)c.page_bytes};
+    const cuuint32_t box[4] = {PG_DIM, KS_KEYS, 1, 1}, ones[4] = {1, 1, 1, 1};
+    const CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, c.data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw Error(JV_ERR_DEVICE, "cuTensorMapEncodeTiled failed with " + std::to_string((int)r));
+    return m;
+}
+
+// The kernel's dynamic shared memory limit, once per kernel and device.
+template <auto kernel>
+void allow_smem(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    JV_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (done.load() & bit) return;
+    JV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit);
+}
+
+template <class T, int NT>
+void launch_small(const AttnKArgs& a, const CUtensorMap& map, int ctas, cudaStream_t s) {
+    allow_smem<k_kv8_small<T, NT>>(KS_SMEM);
+    launch_pdl(k_kv8_small<T, NT>, dim3(ctas), dim3(KS_WARPS * 32), KS_SMEM, s, a, map);
+    note_launch();
 }
 
 template <class T>
@@ -413,15 +791,14 @@ void launch(const AttnKArgs& a, cudaStream_t s) {
     JV_CUDA(cudaGetDevice(&dev));
     JV_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     const int64_t small = a.v.small_cap * a.c.kv_heads, large = a.v.large_cap * a.c.kv_heads;
+    const CUtensorMap map = page_map(a.c);
+    const int ctas = (int)std::min<int64_t>((small + KS_WARPS - 1) / KS_WARPS, (a.rows <= 8 ? 3 : 2) * sms);
     if (a.rows <= 8)
-        k_kv8_small<T, 1><<<(unsigned)std::min<int64_t>(small, 4 * sms), KA_THREADS, 0, s>>>(a);
+        launch_small<T, 1>(a, map, ctas, s);
     else
-        k_kv8_small<T, 2><<<(unsigned)std::min<int64_t>(small, 4 * sms), KA_THREADS, 0, s>>>(a);
-    JV_CUDA(cudaGetLastError());
-    note_launch();
-    if (a.b.max_keys > 256) {
-        k_kv8_join<T><<<dim3(a.b.requests, a.c.kv_heads, a.rows), 256, 0, s>>>(a);
-        JV_CUDA(cudaGetLastError());
+        launch_small<T, 2>(a, map, ctas, s);
+    if (a.b.max_keys > PG_CHUNK) {
+        launch_pdl(k_kv8_join<T>, dim3(small_rows(a.b), a.b.requests, a.c.kv_heads), dim3(KJ_WARPS * 32), 0, s, a);
         note_launch();
     }
     if ((int64_t)a.b.max_new * a.b.group > PG_SMALL_ROWS) {
@@ -479,7 +856,7 @@ int jv_kv8_attention(const jv_kv8_cache* cache, const jv_paged_batch* batch, int
         a.window = window;
         a.part_o = (float*)((char*)ws + w.o);
         a.part_ml = (float2*)((char*)ws + w.ml);
-        a.rows = small_rows(*batch);
+        a.rows = tile_rows(*batch);
         if (type == T_F16)
             launch<__half>(a, (cudaStream_t)stream);
         else

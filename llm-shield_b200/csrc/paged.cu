@@ -43,6 +43,7 @@ void check_cache(const jv_kv8_cache* c) {
     need(c->pages >= 1 && c->kv_heads >= 1 && c->kv_heads <= 1024, "a cache has at least one page and 1 to 1024 KV heads");
     need(c->page_bytes >= (int64_t)c->kv_heads * 2 * PG_PLANE && c->page_bytes % 16 == 0,
          "page_bytes must be a multiple of 16 and at least kv_heads * 16384");
+    need(c->page_bytes < ((int64_t)1 << 40), "page_bytes must be below 2^40");
     need(c->scale_stride >= (int64_t)c->kv_heads * 8 && c->scale_stride % 4 == 0,
          "scale_stride must be a multiple of 4 and at least kv_heads * 8");
     need(aligned(c->data, 16) && aligned(c->scales, 16), "the cache buffers must be 16-byte aligned");
@@ -78,9 +79,13 @@ OnDeviceOf::~OnDeviceOf() {
 PlanView plan_view(const jv_paged_batch& b) {
     PlanView v;
     const int64_t R = b.requests, T = b.max_tokens;
-    // small items: a chunk has at least 256 keys except a request's last; units: every one holds a
+    // small items: a chunk has at least 64 keys except a request's last, 128 where a request has over 32 chunks, and
+    // a request has at most 512 chunks up to 2^19 keys (pg_chunk_keys); units: every one holds a
     // new token, and a request's span has at most new / 16 + 2 of them
-    v.small_cap = R + b.max_keys / 256;
+    const int64_t tiles = (std::min<int64_t>(PG_SMALL_ROWS, (int64_t)b.max_new * b.group) + PG_ROW_TILE - 1) / PG_ROW_TILE;
+    const int64_t most = (int64_t)b.max_blocks * PG_TOKENS;  // of one request's keys
+    const int64_t per = most <= 4096 ? std::min<int64_t>(32, (most + PG_CHUNK - 1) / PG_CHUNK) : std::max<int64_t>(512, (most + 2047) / 2048);
+    v.small_cap = std::min(R + std::min(b.max_keys / PG_CHUNK, 32 * R + b.max_keys / 128), R * per) * tiles;
     v.large_cap = std::min<int64_t>(R, T * b.group / (PG_SMALL_ROWS + 1)) + T * b.group / PG_TILE_ROWS;
     v.unit_cap = std::min<int64_t>(T, T / PG_BLOCK + 2 * R);
     uint8_t* p = (uint8_t*)b.work;
@@ -92,8 +97,8 @@ PlanView plan_view(const jv_paged_batch& b) {
     };
     v.head = (int32_t*)take(8 * 4);
     v.first = (int32_t*)take(R * 4);
-    v.prefix = (int32_t*)take(4 * (R + 1) * 4);
-    v.small_items = (int4*)take(v.small_cap * 16);
+    v.prefix = (int32_t*)take(3 * R * 4);
+    v.small_items = (int4*)take(v.small_cap * 32);
     v.large_items = (int4*)take(v.large_cap * 16);
     v.units = (int2*)take(v.unit_cap * 8);
     v.bytes = at;
@@ -113,224 +118,195 @@ struct PlanArgs {
 };
 
 constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_PER = PG_MAX_REQUESTS / PLAN_THREADS;  // requests per thread at most
+constexpr int PLAN_FILL_THREADS = 128;
+constexpr int PLAN_FILL_REQUESTS = 256;  // most requests that the first launch fills for
 
-// Exclusive sums over the block of five counts per thread; totals in tot.
-__device__ __forceinline__ void block_scan5(int (&x)[5], int (&tot)[5], int (*ws)[5]) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int inc[5];
-#pragma unroll
-    for (int k = 0; k < 5; k++) {
-        inc[k] = x[k];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, inc[k], o);
-            if (lane >= o) inc[k] += y;
-        }
-        if (lane == 31) ws[warp][k] = inc[k];
-    }
-    __syncthreads();
-    if (warp == 0) {
-#pragma unroll
-        for (int k = 0; k < 5; k++) {
-            int y = ws[lane][k];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int z = __shfl_up_sync(0xffffffffu, y, o);
-                if (lane >= o) y += z;
-            }
-            ws[lane][k] = y;
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 5; k++) {
-        tot[k] = ws[31][k];
-        x[k] = (warp ? ws[warp - 1][k] : 0) + inc[k] - x[k];
-    }
+// A request's place in the batch: its lengths and the exclusive sums in front of it.
+struct Place {
+    int old, n_new, start, page, unit, small, large;
+};
+
+__device__ __forceinline__ int units_of(int old, int n_new) {
+    return n_new > 0 ? (old + n_new + PG_BLOCK - 1) / PG_BLOCK - old / PG_BLOCK : 0;
+}
+__device__ __forceinline__ int pages_of(int old, int n_new) {
+    return (old + n_new + PG_TOKENS - 1) / PG_TOKENS - (old + PG_TOKENS - 1) / PG_TOKENS;
+}
+__device__ __forceinline__ bool is_small(int n_new, int group) { return (int64_t)n_new * group <= PG_SMALL_ROWS; }
+__device__ __forceinline__ int small_of(int old, int n_new, int group) {
+    return n_new > 0 && is_small(n_new, group) ? pg_chunks(old + n_new) * ((n_new * group + PG_ROW_TILE - 1) / PG_ROW_TILE) : 0;
+}
+__device__ __forceinline__ int large_of(int n_new, int group) {
+    return n_new > 0 && !is_small(n_new, group) ? (n_new * group + PG_TILE_ROWS - 1) / PG_TILE_ROWS : 0;
 }
 
-__device__ __forceinline__ int tiles_of(int n_new, int group) {
-    return (n_new * group + PG_TILE_ROWS - 1) / PG_TILE_ROWS;
-}
-
-// The last r with prefix[r] <= i, of an exclusive sum prefix[0..n] with prefix[n] > i.
-__device__ __forceinline__ int owner(const int32_t* prefix, int n, int i) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (prefix[mid] <= i) lo = mid; else hi = mid;
-    }
-    return lo;
-}
-
-// Everything but the per-request sums: one thread per token, unit and item, each finding its
-// request by bisection of the exclusive sums (which skips requests that have none).
-__device__ void plan_fill(const PlanArgs& a, int64_t tid, int64_t threads) {
+// One request's pages, tokens, units and items, by threads t, t + n, ...
+__device__ __forceinline__ void plan_request(const PlanArgs& a, int r, const Place& q, int n_free, int t, int n) {
     const jv_paged_batch& b = a.b;
-    const int R = b.requests;
-    const int32_t *unit_pre = a.v.prefix + (R + 1), *small_pre = unit_pre + (R + 1), *large_pre = small_pre + (R + 1);
-    const int tokens = b.starts[R];
-    for (int64_t t = tid; t < tokens; t += threads) {
-        const int r = owner(b.starts, R, (int)t);
-        const int n_new = b.starts[r + 1] - b.starts[r];
-        const int pos = b.lengths[r] - n_new + (int)t - b.starts[r];
-        b.request_of[t] = r;
-        b.positions[t] = pos;
-        b.slots[t] = (int64_t)b.block_table[(int64_t)r * b.max_blocks + pos / PG_TOKENS] * PG_TOKENS + pos % PG_TOKENS;
+    int32_t* row = b.block_table + (int64_t)r * b.max_blocks;
+    const int have = (q.old + PG_TOKENS - 1) / PG_TOKENS, pages = pages_of(q.old, q.n_new);
+    for (int k = t; k < pages; k += n) row[have + k] = a.free_pages[n_free - 1 - (q.page + k)];
+    for (int i = t; i < q.n_new; i += n) {
+        const int pos = q.old + i, blk = pos / PG_TOKENS;
+        // a page of this step comes from where it is taken, so that no thread waits for another's write
+        const int page = blk >= have ? a.free_pages[n_free - 1 - (q.page + blk - have)] : row[blk];
+        b.request_of[q.start + i] = r;
+        b.positions[q.start + i] = pos;
+        b.slots[q.start + i] = (int64_t)page * PG_TOKENS + pos % PG_TOKENS;
     }
-    for (int64_t i = tid; i < unit_pre[R]; i += threads) {
-        const int r = owner(unit_pre, R, (int)i);
-        const int old = b.lengths[r] - (b.starts[r + 1] - b.starts[r]);
-        a.v.units[i] = make_int2(r, old / PG_BLOCK + (int)i - unit_pre[r]);
+    const int units = units_of(q.old, q.n_new);
+    for (int i = t; i < units; i += n) a.v.units[q.unit + i] = make_int2(r, q.old / PG_BLOCK + i);
+    const int small = small_of(q.old, q.n_new, b.group), chunks = pg_chunks(q.old + q.n_new);
+    for (int i = t; i < small; i += n) {
+        a.v.small_items[2 * (q.small + i)] = make_int4(r, i % chunks, chunks, i / chunks);
+        a.v.small_items[2 * (q.small + i) + 1] = make_int4(q.start, q.n_new, q.old + q.n_new, 0);
     }
-    for (int64_t i = tid; i < small_pre[R]; i += threads) {
-        const int r = owner(small_pre, R, (int)i);
-        a.v.small_items[i] = make_int4(r, (int)i - small_pre[r], small_pre[r + 1] - small_pre[r], 0);
-    }
-    for (int64_t i = tid; i < large_pre[R]; i += threads) {
-        const int r = owner(large_pre, R, (int)i);
-        // a request's last tile sees the most keys: first
-        a.v.large_items[i] = make_int4(r, large_pre[r + 1] - 1 - (int)i, 0, 0);
-    }
+    const int large = large_of(q.n_new, b.group);
+    // a request's last tile sees the most keys: first
+    for (int i = t; i < large; i += n) a.v.large_items[q.large + i] = make_int4(r, large - 1 - i, 0, 0);
 }
 
-// One CTA: the sums over the requests, the checks, the new pages. Latency-bound: each thread holds
-// up to 4 consecutive requests, one block-wide scan of five counts.
+// One CTA: the sums over the requests and the checks; with `fill`, everything else too, a warp per
+// request. Latency-bound: each thread holds up to 4 consecutive requests, the sums are one pass of
+// warp shuffles and one barrier (every warp adds up the warps' totals for itself).
 __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
     __shared__ int ws[32][5];
-    __shared__ unsigned long long keys_total, token_total;
-    __shared__ int bad_code, bad_site;
+    __shared__ long long wl[32][2];
+    __shared__ Place places[PLAN_FILL_REQUESTS];
     const jv_paged_batch& b = a.b;
-    const int R = b.requests, tid = threadIdx.x;
-    if (tid == 0) {
-        keys_total = token_total = 0;
-        bad_code = bad_site = 0;
-    }
-    __syncthreads();
-    const int per = (R + PLAN_THREADS - 1) / PLAN_THREADS;  // <= 4
-    const int r0 = tid * per;
-    int old[4], n_new[4], cnt[4][5], sum[5] = {0, 0, 0, 0, 0};
+    const int R = b.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    const int per = (R + blockDim.x - 1) / blockDim.x, r0 = tid * per;  // per <= PLAN_PER
+    const int n_free = *a.n_free;
+    int old[PLAN_PER], n_new[PLAN_PER], sum[5] = {0, 0, 0, 0, 0};
     long long keys = 0, tokens = 0;
     bool bad = false;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        old[j] = n_new[j] = 0;
-        if (j < per && r0 + j < R) {
-            old[j] = a.cached[r0 + j];
-            n_new[j] = a.new_tokens[r0 + j];
+    for (int j = 0; j < PLAN_PER; j++) {
+        const bool in = j < per && r0 + j < R;
+        old[j] = in ? a.cached[r0 + j] : 0;
+        n_new[j] = in ? a.new_tokens[r0 + j] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < PLAN_PER; j++) {
+        const long long total = (long long)old[j] + n_new[j];
+        if (old[j] < 0 || n_new[j] < 0 || n_new[j] > b.max_new || total > (long long)b.max_blocks * PG_TOKENS) {
+            bad = true;  // the step fails; its counts are left out
+            continue;
         }
-        if (old[j] < 0 || n_new[j] < 0 || n_new[j] > b.max_new ||
-            (long long)old[j] + n_new[j] > (long long)b.max_blocks * PG_TOKENS)
-            bad = true;
-        keys += (long long)old[j] + n_new[j];
+        keys += total;
         tokens += n_new[j];
+        sum[0] += n_new[j];
+        sum[1] += pages_of(old[j], n_new[j]);
+        sum[2] += units_of(old[j], n_new[j]);
+        sum[3] += small_of(old[j], n_new[j], b.group);
+        sum[4] += large_of(n_new[j], b.group);
     }
-    if (bad) {
-        if (atomicCAS(&bad_code, 0, JV_ERR_RANGE) == 0) bad_site = PS_PLAN_LENGTH;
-        keys = tokens = 0;
-    }
-    atomicAdd(&keys_total, (unsigned long long)keys);
-    atomicAdd(&token_total, (unsigned long long)tokens);
-    __syncthreads();
-    if (tid == 0 && bad_code == 0) {
-        if (token_total > (unsigned long long)b.max_tokens) {
-            bad_code = JV_ERR_RANGE;
-            bad_site = PS_PLAN_TOKENS;
-        } else if (keys_total > (unsigned long long)b.max_keys) {
-            bad_code = JV_ERR_RANGE;
-            bad_site = PS_PLAN_KEYS;
+    int pre[5];
+#pragma unroll
+    for (int k = 0; k < 5; k++) {
+        int x = sum[k];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
         }
+        if (lane == 31) ws[warp][k] = x;
+        pre[k] = x - sum[k];
     }
-    __syncthreads();
-    const bool within = bad_code == 0;  // from here on every count fits its list
-    const int n_free = *a.n_free;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int o = 16; o >= 1; o >>= 1) {
+        keys += __shfl_xor_sync(0xffffffffu, keys, o);
+        tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
+    }
+    if (lane == 0) wl[warp][0] = keys, wl[warp][1] = tokens;
+    bad = __syncthreads_or(bad);
+    int tot[5];
+    {
+        int before[5];
 #pragma unroll
-        for (int k = 0; k < 5; k++) cnt[j][k] = 0;
-        const int total = old[j] + n_new[j];
-        if (!within || j >= per || r0 + j >= R) continue;
-        cnt[j][0] = n_new[j];
-        cnt[j][1] = (total + PG_TOKENS - 1) / PG_TOKENS - (old[j] + PG_TOKENS - 1) / PG_TOKENS;
-        if (n_new[j] > 0) {
-            cnt[j][2] = (total + PG_BLOCK - 1) / PG_BLOCK - old[j] / PG_BLOCK;
-            if ((int64_t)n_new[j] * b.group <= PG_SMALL_ROWS)
-                cnt[j][3] = pg_chunks(total);
-            else
-                cnt[j][4] = tiles_of(n_new[j], b.group);
+        for (int k = 0; k < 5; k++) {
+            const int x = lane < warps ? ws[lane][k] : 0;
+            before[k] = lane < warp ? x : 0;
+            tot[k] = x;
         }
+        keys = lane < warps ? wl[lane][0] : 0;
+        tokens = lane < warps ? wl[lane][1] : 0;
 #pragma unroll
-        for (int k = 0; k < 5; k++) sum[k] += cnt[j][k];
-    }
-    int tot[5], pre[5];
+        for (int o = 16; o >= 1; o >>= 1) {
 #pragma unroll
-    for (int k = 0; k < 5; k++) pre[k] = sum[k];
-    block_scan5(pre, tot, ws);
-    if (tid == 0 && within && (n_free < 0 || tot[1] > n_free)) {
-        bad_code = JV_ERR_OOM;
-        bad_site = PS_PLAN_FREE;
-    }
-    __syncthreads();
-    if (bad_code == 0)
-        for (int i = tid; i < tot[1]; i += PLAN_THREADS)
-            if ((unsigned)a.free_pages[n_free - 1 - i] >= (unsigned)b.pages) {
-                atomicExch(&bad_site, PS_PLAN_PAGE);
-                atomicExch(&bad_code, JV_ERR_RANGE);
+            for (int k = 0; k < 5; k++) {
+                before[k] += __shfl_xor_sync(0xffffffffu, before[k], o);
+                tot[k] += __shfl_xor_sync(0xffffffffu, tot[k], o);
             }
-    __syncthreads();
-    const bool ok = bad_code == 0;
-    int32_t *page_pre = a.v.prefix, *unit_pre = page_pre + (R + 1), *small_pre = unit_pre + (R + 1),
-            *large_pre = small_pre + (R + 1);
+            keys += __shfl_xor_sync(0xffffffffu, keys, o);
+            tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
+        }
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+        for (int k = 0; k < 5; k++) pre[k] += before[k];
+    }
+    int code = 0, site = 0;  // the same in every thread
+    if (bad)
+        code = JV_ERR_RANGE, site = PS_PLAN_LENGTH;
+    else if (tokens > b.max_tokens)
+        code = JV_ERR_RANGE, site = PS_PLAN_TOKENS;
+    else if (keys > b.max_keys)
+        code = JV_ERR_RANGE, site = PS_PLAN_KEYS;
+    else if (n_free < 0 || tot[1] > n_free)
+        code = JV_ERR_OOM, site = PS_PLAN_FREE;
+    if (code == 0) {
+        bool out = false;
+        for (int i = tid; i < tot[1]; i += blockDim.x) out |= (unsigned)a.free_pages[n_free - 1 - i] >= (unsigned)b.pages;
+        if (__syncthreads_or(out)) code = JV_ERR_RANGE, site = PS_PLAN_PAGE;
+    }
+    const bool ok = code == 0;
+    int32_t* prefix = a.v.prefix;
+#pragma unroll
+    for (int j = 0; j < PLAN_PER; j++) {
         const int r = r0 + j;
         if (j >= per || r >= R) continue;
-        b.lengths[r] = ok ? old[j] + n_new[j] : old[j];
-        b.starts[r] = ok ? pre[0] : 0;
-        page_pre[r] = ok ? pre[1] : 0;
-        unit_pre[r] = ok ? pre[2] : 0;
-        small_pre[r] = ok ? pre[3] : 0;
-        large_pre[r] = ok ? pre[4] : 0;
-        a.v.first[r] = ok ? pre[3] : 0;
-        if (ok) {
-            const int have = (old[j] + PG_TOKENS - 1) / PG_TOKENS;
-            // a request that takes many pages is served by the whole block below
-            if (cnt[j][1] <= 4)
-                for (int k = 0; k < cnt[j][1]; k++)
-                    b.block_table[(int64_t)r * b.max_blocks + have + k] = a.free_pages[n_free - 1 - (pre[1] + k)];
+        const Place q = {old[j], ok ? n_new[j] : 0, ok ? pre[0] : 0, ok ? pre[1] : 0, ok ? pre[2] : 0, ok ? pre[3] : 0, ok ? pre[4] : 0};
+        b.lengths[r] = q.old + q.n_new;
+        b.starts[r] = q.start;
+        a.v.first[r] = q.small;
+        if (fill) {
+            places[r] = q;
+        } else {
+            prefix[r] = q.page;
+            prefix[R + r] = q.unit;
+            prefix[2 * R + r] = q.large;
         }
-#pragma unroll
-        for (int k = 0; k < 5; k++) pre[k] += cnt[j][k];
+        pre[0] += n_new[j];
+        pre[1] += pages_of(old[j], n_new[j]);
+        pre[2] += units_of(old[j], n_new[j]);
+        pre[3] += small_of(old[j], n_new[j], b.group);
+        pre[4] += large_of(n_new[j], b.group);
     }
     if (tid == 0) {
         b.starts[R] = ok ? tot[0] : 0;
-        page_pre[R] = ok ? tot[1] : 0;
-        unit_pre[R] = ok ? tot[2] : 0;
-        small_pre[R] = ok ? tot[3] : 0;
-        large_pre[R] = ok ? tot[4] : 0;
         a.v.head[0] = ok ? tot[3] : 0;
         a.v.head[1] = ok ? tot[4] : 0;
         a.v.head[2] = ok ? tot[2] : 0;
+        a.v.head[3] = n_free;
         *a.n_free_out = ok ? n_free - tot[1] : n_free;
-        if (!ok) paged_report(b.status, bad_code, bad_site);
+        if (!ok) paged_report(b.status, code, site);
     }
-    __syncthreads();
-    if (ok)
-        for (int i = tid; i < tot[1]; i += PLAN_THREADS) {
-            const int r = owner(page_pre, R, i);
-            if (page_pre[r + 1] - page_pre[r] <= 4) continue;  // written above
-            const int old_len = b.lengths[r] - (b.starts[r + 1] - b.starts[r]);
-            b.block_table[(int64_t)r * b.max_blocks + (old_len + PG_TOKENS - 1) / PG_TOKENS + i - page_pre[r]] =
-                a.free_pages[n_free - 1 - i];
-        }
-    if (fill) {
+    if (fill && ok) {
         __syncthreads();
-        plan_fill(a, tid, PLAN_THREADS);
+        for (int r = warp; r < R; r += warps)
+            if (places[r].n_new > 0) plan_request(a, r, places[r], n_free, lane, 32);
     }
 }
 
-__global__ void __launch_bounds__(256) k_plan_fill(PlanArgs a) {
-    plan_fill(a, (int64_t)blockIdx.x * blockDim.x + threadIdx.x, (int64_t)gridDim.x * blockDim.x);
+// The rest of a larger step: a CTA per request and slice of its tokens.
+__global__ void __launch_bounds__(PLAN_FILL_THREADS) k_plan_fill(PlanArgs a) {
+    pdl_wait();
+    const jv_paged_batch& b = a.b;
+    const int r = blockIdx.x, R = b.requests;
+    const int len = b.lengths[r], start = b.starts[r], n_new = b.starts[r + 1] - start;
+    const Place q = {len - n_new, n_new, start, a.v.prefix[r], a.v.prefix[R + r], a.v.first[r], a.v.prefix[2 * R + r]};
+    const int n_free = a.v.head[3];
+    if (n_new > 0) plan_request(a, r, q, n_free, blockIdx.y * PLAN_FILL_THREADS + threadIdx.x, gridDim.y * PLAN_FILL_THREADS);
 }
 
 // ------------------------------------------------------------ read-back
@@ -419,17 +395,16 @@ int jv_paged_plan(const jv_paged_batch* batch, const int32_t* cached, const int3
         if (!cached || !new_tokens || !free_pages || !n_free || !n_free_out) throw Error(JV_ERR_ARG, "NULL buffer");
         OnDeviceOf dev(batch->work);
         PlanArgs a{*batch, plan_view(*batch), cached, new_tokens, free_pages, n_free, n_free_out};
-        // One CTA fills the arrays too where they are short enough that a second launch would cost
-        // more than its parallelism saves.
-        const int64_t rows = a.v.unit_cap + a.v.small_cap + a.v.large_cap + batch->max_tokens;
-        const bool fill = rows <= 4096;
-        k_plan<<<1, PLAN_THREADS, 0, (cudaStream_t)stream>>>(a, fill);
+        // A CTA of few warps for few requests. It fills the arrays too where a warp per request gets
+        // through them in less than a second launch costs (16 requests of one token: 3.9 us in one launch).
+        const bool fill = batch->requests <= PLAN_FILL_REQUESTS && batch->max_new <= 256 && batch->max_tokens <= 4096;
+        const int threads = batch->requests <= 8 ? 256 : PLAN_THREADS;
+        k_plan<<<1, threads, 0, (cudaStream_t)stream>>>(a, fill);
         JV_CUDA(cudaGetLastError());
         note_launch();
         if (!fill) {
-            const int64_t ctas = std::min<int64_t>((batch->max_tokens + 255) / 256, 4 * 148);
-            k_plan_fill<<<(unsigned)ctas, 256, 0, (cudaStream_t)stream>>>(a);
-            JV_CUDA(cudaGetLastError());
+            const int slices = std::min(32, (batch->max_new + 1023) / 1024);
+            launch_pdl(k_plan_fill, dim3(batch->requests, slices), dim3(PLAN_FILL_THREADS), 0, (cudaStream_t)stream, a);
             note_launch();
         }
     });

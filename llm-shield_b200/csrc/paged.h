@@ -13,27 +13,33 @@ constexpr int PG_PLANE = PG_TOKENS * PG_DIM;       // bytes of one K or V plane 
 constexpr int PG_MAX_REQUESTS = 4096;
 constexpr int PG_MAX_GROUP = 16;
 
-// A request whose new tokens x group give at most this many query rows is "small": its keys are
-// split into chunks that different CTAs take (kv8_attn.cu). The others go by tiles of query rows.
-constexpr int PG_SMALL_ROWS = 16;
+// A request whose new tokens x group give at most PG_SMALL_ROWS query rows is "small": its keys are
+// split into chunks that different CTAs take, PG_ROW_TILE rows at a time (kv8_attn.cu). The others go by
+// tiles of query rows over all their keys.
+constexpr int PG_SMALL_ROWS = 32;
+constexpr int PG_ROW_TILE = 16;
 constexpr int PG_TILE_ROWS = 16;
-constexpr int PG_MAX_CHUNKS = 128;
 
-// Keys per chunk of a small request: 256, or as many more as keep the chunks at 128 at most.
-// It goes by the request's own length, so a request is cut alike in every batch.
+// Keys per chunk of a small request: 64 up to 2048 keys, where latency counts; then as many as keep what a
+// chunk leaves behind (rows x 528 bytes, written and read again) small against its keys. It goes by the
+// request's own length, so a request is cut alike in every batch. Always a multiple of 64, at most 2048
+// (32 pages: one per lane).
+constexpr int PG_CHUNK = 64;
 __host__ __device__ inline int pg_chunk_keys(int len) {
-    return 256 * ((len + 256 * PG_MAX_CHUNKS - 1) / (256 * PG_MAX_CHUNKS));
+    if (len <= 2048) return PG_CHUNK;
+    if (len <= 4096) return 128;
+    return len <= 131072 ? 256 : len <= 524288 ? 1024 : 2048;
 }
 __host__ __device__ inline int pg_chunks(int len) {
-    return len <= 0 ? 0 : (len + pg_chunk_keys(len) - 1) / pg_chunk_keys(len);
+    return len <= 0 ? 0 : (int)(((int64_t)len + pg_chunk_keys(len) - 1) / pg_chunk_keys(len));
 }
 
 // A plan's work lists, in jv_paged_batch.work.
 struct PlanView {
-    int32_t* head;      // [8]: small items, large items, append units
+    int32_t* head;      // [8]: small items, large items, append units, free pages before the step
     int32_t* first;     // [requests] first small item of each request
-    int32_t* prefix;    // [4][requests + 1]: needed pages, units, small items, large items before request r
-    int4* small_items;  // {request, chunk, chunks, 0}
+    int32_t* prefix;    // [3][requests]: pages taken, units and large items before request r
+    int4* small_items;  // two each: {request, chunk, chunks, row tile}, {start, new, length, 0}; row tile by row tile
     int4* large_items;  // {request, tile, 0, 0}
     int2* units;        // {request, block}: the 16-token blocks the step writes to
     int64_t small_cap, large_cap, unit_cap, bytes;
@@ -71,7 +77,7 @@ int paged_api(F&& f) {
 enum PagedSite : int {
     PS_PLAN_LENGTH = 96, PS_PLAN_TOKENS = 97, PS_PLAN_KEYS = 98, PS_PLAN_FREE = 99, PS_PLAN_PAGE = 100,
     PS_APPEND_PAGE = 101, PS_APPEND_VALUE = 102, PS_READ_SLOT = 103, PS_READ_VALUE = 104, PS_ATTN_REQUEST = 105,
-    PS_ATTN_PAGE = 106, PS_ROPE_VALUE = 107
+    PS_ATTN_PAGE = 106, PS_ROPE_VALUE = 107, PS_ATTN_WAIT = 108
 };
 
 #ifdef __CUDACC__
@@ -85,13 +91,16 @@ __device__ __forceinline__ void paged_report(int32_t* status, int code, int site
 struct RequestRows {
     int start, n_new, len;
 };
+__device__ __forceinline__ bool rows_in_bounds(const jv_paged_batch& b, int start, int n_new, int len) {
+    return start >= 0 && n_new >= 0 && n_new <= b.max_new && start <= b.max_tokens - n_new && len >= 0 &&
+           len <= (int64_t)b.max_blocks * PG_TOKENS;
+}
 __device__ __forceinline__ bool request_rows(const jv_paged_batch& b, int r, RequestRows& o) {
     if (r < 0 || r >= b.requests) return false;
     o.start = b.starts[r];
     o.n_new = b.starts[r + 1] - o.start;
     o.len = b.lengths[r];
-    return o.start >= 0 && o.n_new >= 0 && o.n_new <= b.max_new && o.start <= b.max_tokens - o.n_new && o.len >= 0 &&
-           o.len <= (int64_t)b.max_blocks * PG_TOKENS;
+    return rows_in_bounds(b, o.start, o.n_new, o.len);
 }
 #endif
 
