@@ -33,7 +33,8 @@ NVCC_FLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-
                      "-Xcompiler", "-Wall,-Wno-unused-function", "-I", str(PKG.parent / "include")]
 
 SOURCES = ["gguf.cpp", "qx.cpp", "runtime.cu", "kernels_quant.cu", "kernels_elem.cu", "kernels_attn.cu", "attn_tc.cu", "gemm_tc.cu",
-           "quantmatmul.cu", "noalloc.cu", "kernels_decode.cu", "paged.cu", "kernels_rope.cu", "kv8_attn.cu"]
+           "quantmatmul.cu", "noalloc.cu", "kernels_decode.cu", "paged.cu", "kernels_rope.cu", "kv8_attn.cu",
+           "kv8_attn_tc.cu"]
 
 
 def _run(cmd: list[str], verbose: bool) -> str:

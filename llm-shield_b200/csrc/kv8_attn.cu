@@ -7,6 +7,7 @@
 // int8 is exact in fp16), w_j <= 2^8 is the only rounded operand (fp16, half a step 2^-12), and sums, M
 // and the softmax denominator are fp32. bf16 queries are taken to fp16 by a power of two per row.
 //
+// Here: the requests of few query rows, whose time is the cache's bytes. (kv8_attn_tc.cu has the others.)
 // The products are mma.sync m16n8k16 with the keys on the 16-row side and the query rows (new token x
 // head of the group) on the 8-column side: S^T = K Q^T, O^T = V^T P^T. The order of the 128
 // dimensions inside a product is free, so a lane loads 16 consecutive int8 of its rows straight from
@@ -24,27 +25,7 @@
 namespace jv {
 namespace {
 
-constexpr int KA_WARPS = 4;
-constexpr int KA_THREADS = KA_WARPS * 32;
 constexpr float KA_LOG2E = 1.4426950408889634f;
-
-struct AttnKArgs {
-    jv_kv8_cache c;
-    jv_paged_batch b;
-    PlanView v;
-    jv_heads q;
-    float scale;  // times log2 e
-    int window;
-    float* part_o;   // [small item][kv head][rows][128]
-    float2* part_ml; // [small item][kv head][rows]
-    int rows;        // query rows of a small item's partials
-};
-
-__device__ __forceinline__ float ex2f(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
 
 __device__ __forceinline__ float lg2f(float x) {
     float y;
@@ -105,194 +86,6 @@ __device__ __forceinline__ float q_to_f16(uint32_t (&q)[16]) {
         q[e] = pack2<__half>(x.x * up, x.y * up);
     }
     return up;
-}
-
-// Rows [row0, row0 + 8 NT) of a request's query rows (row = new token * group + head of the group)
-// against keys [k_lo, k_hi) of one KV head, by one CTA. The warps take the 16-key tiles in turn and
-// are joined in shared memory. Leaves acc / m / l joined in shared memory: O[row][dim], ml[row].
-template <class T, int NT>
-struct Smem {
-    float o[KA_WARPS][8 * NT][PG_DIM + 4];
-    float m[KA_WARPS][8 * NT], l[KA_WARPS][8 * NT];
-};
-
-template <class T, int NT>
-__device__ __forceinline__ void attend(const AttnKArgs& a, Smem<T, NT>& sm, const RequestRows& rr, int request, int kvh,
-                                       int row0, int k_lo, int k_hi) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, i = lane & 3;
-    const int group = a.b.group, n_rows = rr.n_new * group;
-    // B fragments of Q^T: lane (g, i) holds row g's dimensions 16 i .. + 15 and 64 + 16 i .. + 15
-    uint32_t qf[NT][16];
-    float qs[NT][2];         // per accumulator column 2 i, 2 i + 1: the scale of its row
-    int lo_key[NT][2], hi_key[NT][2];  // visible keys of that row
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int row = row0 + 8 * n + g;
-        float f = 1.f;
-        if (row < n_rows) {
-            const T* src = (const T*)a.q.in + (int64_t)(rr.start + row / group) * a.q.in_token +
-                           (int64_t)(kvh * group + row % group) * a.q.in_head + 16 * i;
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const uint4 x = *(const uint4*)(src + 64 * j + 8 * e);
-                    qf[n][8 * j + 4 * e] = x.x, qf[n][8 * j + 4 * e + 1] = x.y;
-                    qf[n][8 * j + 4 * e + 2] = x.z, qf[n][8 * j + 4 * e + 3] = x.w;
-                }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 16; e++) qf[n][e] = 0;
-        }
-        if (std::is_same<T, __nv_bfloat16>::value) f = 1.f / q_to_f16(qf[n]);
-        f *= a.scale;
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int col = 2 * i + e, r = row0 + 8 * n + col;
-            qs[n][e] = __shfl_sync(0xffffffffu, f, 4 * col);
-            const int pos = rr.len - rr.n_new + r / group;
-            hi_key[n][e] = r < n_rows ? pos + 1 : 0;
-            lo_key[n][e] = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-        }
-    }
-    float acc[NT][8][4], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        m[n][0] = m[n][1] = -INFINITY;
-        l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) acc[n][j][e] = 0.f;
-    }
-    const int32_t* table = a.b.block_table + (int64_t)request * a.b.max_blocks;
-    for (int t = k_lo / PG_BLOCK + warp; t * PG_BLOCK < k_hi; t += KA_WARPS) {
-        const int key0 = t * PG_BLOCK;
-        const int page = table[key0 / PG_TOKENS];
-        if ((unsigned)page >= (unsigned)a.c.pages) {
-            if (lane == 0) paged_report(a.b.status, JV_ERR_RANGE, PS_ATTN_PAGE);
-            continue;
-        }
-        const char* kp = (const char*)a.c.data + (int64_t)page * a.c.page_bytes + (int64_t)kvh * 2 * PG_PLANE +
-                         (key0 % PG_TOKENS) * PG_DIM;
-        const char* vp = kp + PG_PLANE;
-        const float* sp = a.c.scales + (int64_t)page * a.c.scale_stride + kvh * 8 + (key0 % PG_TOKENS) / PG_BLOCK;
-        const float ks = sp[0];
-        float vs = sp[4];
-        uint4 kr[2][2], vr[4];
-#pragma unroll
-        for (int r = 0; r < 2; r++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) kr[r][j] = *(const uint4*)(kp + (g + 8 * r) * PG_DIM + 64 * j + 16 * i);
-#pragma unroll
-        for (int r = 0; r < 4; r++) vr[r] = *(const uint4*)(vp + (2 * i + (r & 1) + 8 * (r >> 1)) * PG_DIM + 16 * g);
-        if (!(vs > 0.f)) vs = 1.f;  // a block of zeros
-        const float lvs = log2f(vs), ivs = 1.f / vs;
-        // S^T
-        float s[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[n][e] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const uint32_t w0[4] = {kr[0][j].x, kr[0][j].y, kr[0][j].z, kr[0][j].w};
-            const uint32_t w1[4] = {kr[1][j].x, kr[1][j].y, kr[1][j].z, kr[1][j].w};
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const uint32_t x0 = w0[w] ^ 0x80808080u, x1 = w1[w] ^ 0x80808080u;
-                const uint32_t f[4] = {pair_f16(x0, 0x4140), pair_f16(x1, 0x4140), pair_f16(x0, 0x4342), pair_f16(x1, 0x4342)};
-#pragma unroll
-                for (int n = 0; n < NT; n++) mma_f16(s[n], f, qf[n][8 * j + 2 * w], qf[n][8 * j + 2 * w + 1]);
-            }
-        }
-        uint32_t pb[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            float e[4], mx[2];
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int key = key0 + g + 8 * (x >> 1), c = x & 1;
-                e[x] = fmaf(s[n][x], ks * qs[n][c], lvs);
-                if (key >= hi_key[n][c] || key < lo_key[n][c]) e[x] = -INFINITY;
-            }
-            float alpha[2];
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                mx[c] = fmaxf(e[c], e[c + 2]);
-                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
-                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 8));
-                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 16));
-                const float mn = fmaxf(m[n][c], mx[c]);
-                const float ref = mn == -INFINITY ? 0.f : mn;
-                alpha[c] = ex2f(m[n][c] - ref);
-                m[n][c] = mn;
-                e[c] = ex2f(e[c] - ref);
-                e[c + 2] = ex2f(e[c + 2] - ref);
-                l[n][c] = fmaf(l[n][c], alpha[c], (e[c] + e[c + 2]) * ivs);
-            }
-            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-#pragma unroll
-                    for (int x = 0; x < 4; x++) acc[n][j][x] *= alpha[x & 1];
-            }
-            pb[n][0] = movmatrix_trans(pack2<__half>(e[0], e[1]));
-            pb[n][1] = movmatrix_trans(pack2<__half>(e[2], e[3]));
-        }
-        // O^T += V^T P^T: dimension 16 g + 2 j is the tile's row g, 16 g + 2 j + 1 its row g + 8
-        const uint32_t va[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w}, vb[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
-        const uint32_t vc[4] = {vr[2].x, vr[2].y, vr[2].z, vr[2].w}, vd[4] = {vr[3].x, vr[3].y, vr[3].z, vr[3].w};
-#pragma unroll
-        for (int w = 0; w < 4; w++)
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const uint32_t sel = u ? 0x7362 : 0x5140;
-                const uint32_t lo = __byte_perm(va[w], vb[w], sel) ^ 0x80808080u, hi = __byte_perm(vc[w], vd[w], sel) ^ 0x80808080u;
-                const uint32_t f[4] = {pair_f16(lo, 0x4140), pair_f16(lo, 0x4342), pair_f16(hi, 0x4140), pair_f16(hi, 0x4342)};
-#pragma unroll
-                for (int n = 0; n < NT; n++) mma_f16(acc[n][2 * w + u], f, pb[n][0], pb[n][1]);
-            }
-    }
-    // join the warps
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 4);
-            l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 8);
-            l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 16);
-            const int row = 8 * n + 2 * i + c;
-            if (g == 0) {
-                sm.m[warp][row] = m[n][c];
-                sm.l[warp][row] = l[n][c];
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                float2* dst = (float2*)&sm.o[warp][row][16 * g + 2 * j];
-                *dst = make_float2(acc[n][j][c], acc[n][j][c + 2]);
-            }
-        }
-    __syncthreads();
-}
-
-// Row r of the joined warps, dimensions 4 d4 .. + 3: unnormalised values, reference and denominator.
-template <class T, int NT>
-__device__ __forceinline__ float4 joined(const Smem<T, NT>& sm, int r, int d4, float& m, float& l) {
-    m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < KA_WARPS; w++) m = fmaxf(m, sm.m[w][r]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    l = 0.f;
-#pragma unroll
-    for (int w = 0; w < KA_WARPS; w++) {
-        const float f = ex2f(sm.m[w][r] - ref);
-        const float4 x = *(const float4*)&sm.o[w][r][4 * d4];
-        l = fmaf(sm.l[w][r], f, l);
-        o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
-    }
-    return o;
 }
 
 template <class T>
@@ -563,7 +356,7 @@ __global__ void __launch_bounds__(KS_WARPS * 32, NT == 1 ? 3 : 2) k_kv8_small(At
 #pragma unroll
                             for (int c = 0; c < 2; c++) {
                                 const float mn = fmaxf(m[n][c], mx[c]);
-                                alpha[c] = m[n][c] == -INFINITY ? 0.f : ex2f(m[n][c] - mn);
+                                alpha[c] = m[n][c] == -INFINITY ? 0.f : ex2(m[n][c] - mn);
                                 m[n][c] = mn;
                                 l[n][c] *= alpha[c];
                             }
@@ -577,8 +370,8 @@ __global__ void __launch_bounds__(KS_WARPS * 32, NT == 1 ? 3 : 2) k_kv8_small(At
 #pragma unroll
                             for (int c = 0; c < 2; c++) {
                                 const float ref = m[n][c] == -INFINITY ? 0.f : m[n][c];
-                                e[h][c] = ex2f(e[h][c] - ref);
-                                e[h][c + 2] = ex2f(e[h][c + 2] - ref);
+                                e[h][c] = ex2(e[h][c] - ref);
+                                e[h][c + 2] = ex2(e[h][c + 2] - ref);
                                 l[n][c] = fmaf(e[h][c] + e[h][c + 2], iv[h], l[n][c]);
                             }
                             pb[h][n][0] = movmatrix_trans(pack2<__half>(e[h][0], e[h][1]));
@@ -677,13 +470,13 @@ __global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
             x[k] = in ? *(const float4*)(a.part_o + (p0 + c * step) * PG_DIM + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         const float mn = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
-        const float ref = mn == -INFINITY ? 0.f : mn, f0 = ex2f(m - ref);
+        const float ref = mn == -INFINITY ? 0.f : mn, f0 = ex2(m - ref);
         m = mn;
         l *= f0;
         o.x *= f0, o.y *= f0, o.z *= f0, o.w *= f0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const float f = ex2f(ml[k].x - ref);
+            const float f = ex2(ml[k].x - ref);
             l = fmaf(ml[k].y, f, l);
             o.x = fmaf(x[k].x, f, o.x), o.y = fmaf(x[k].y, f, o.y), o.z = fmaf(x[k].z, f, o.z), o.w = fmaf(x[k].w, f, o.w);
         }
@@ -700,7 +493,7 @@ __global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
     l = 0.f;
 #pragma unroll
     for (int w = 0; w < KJ_WARPS; w++) {
-        const float f = ex2f(sl[w].x - ref);
+        const float f = ex2(sl[w].x - ref);
         const float4 x = so[w][lane];
         l = fmaf(sl[w].y, f, l);
         o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
@@ -708,41 +501,23 @@ __global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
     store_row<T>(a, rr.start, kvh, row, lane, o, l);
 }
 
-// Large requests: one CTA per (tile of 16 query rows, KV head), over all its keys.
-template <class T>
-__global__ void __launch_bounds__(KA_THREADS) k_kv8_large(AttnKArgs a) {
-    __shared__ __align__(16) Smem<T, 2> sm;
-    const int kvh_n = a.c.kv_heads;
-    const int64_t n = (int64_t)min((int64_t)max(a.v.head[1], 0), a.v.large_cap) * kvh_n;
-    for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
-        const int kvh = (int)(w % kvh_n);
-        const int4 it = a.v.large_items[w / kvh_n];
-        RequestRows rr;
-        if (!request_rows(a.b, it.x, rr)) continue;
-        const int n_rows = rr.n_new * a.b.group, row0 = it.y * PG_TILE_ROWS;
-        if (row0 < 0 || row0 >= n_rows) continue;
-        const int rows = min(PG_TILE_ROWS, n_rows - row0);
-        const int first = rr.len - rr.n_new + row0 / a.b.group, last = rr.len - rr.n_new + (row0 + rows - 1) / a.b.group;
-        attend<T, 2>(a, sm, rr, it.x, kvh, row0, a.window > 0 ? max(0, first + 1 - a.window) : 0, max(0, last + 1));
-        for (int e = threadIdx.x; e < rows * 32; e += KA_THREADS) {
-            float m, l;
-            const float4 o = joined<T, 2>(sm, e >> 5, e & 31, m, l);
-            store_row<T>(a, rr.start, kvh, row0 + (e >> 5), e & 31, o, l);
-        }
-        __syncthreads();
-    }
-}
-
 // Query rows of a small item, and row tiles of a small request, at most.
 int tile_rows(const jv_paged_batch& b) { return (int)std::min<int64_t>(PG_ROW_TILE, (int64_t)b.max_new * b.group); }
 int small_rows(const jv_paged_batch& b) { return (int)std::min<int64_t>(PG_SMALL_ROWS, (int64_t)b.max_new * b.group); }
 
 struct Workspace {
-    int64_t o, ml, bytes;
+    int64_t o, ml, large_o, large_ml, bytes;
 };
 Workspace workspace(const jv_paged_batch& b, int kv_heads) {
-    const int64_t n = plan_view(b).small_cap * kv_heads * tile_rows(b);
-    return {0, n * PG_DIM * 4, n * (PG_DIM * 4 + 8)};
+    const PlanView v = plan_view(b);
+    const int64_t small = v.small_cap * kv_heads * tile_rows(b), large = v.split_cap * kv_heads * 2 * PG_TILE;
+    Workspace w;
+    w.o = 0;
+    w.ml = small * PG_DIM * 4;
+    w.large_o = (w.ml + small * 8 + 15) & ~(int64_t)15;
+    w.large_ml = w.large_o + large * PG_DIM * 4;
+    w.bytes = w.large_ml + large * 8;
+    return w;
 }
 
 // The cache as a 4-dimensional tensor of bytes, [page][kv head][K rows, V rows][128]; a box is the K or
@@ -790,7 +565,7 @@ void launch(const AttnKArgs& a, cudaStream_t s) {
     int sms = 148, dev = 0;
     JV_CUDA(cudaGetDevice(&dev));
     JV_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    const int64_t small = a.v.small_cap * a.c.kv_heads, large = a.v.large_cap * a.c.kv_heads;
+    const int64_t small = a.v.small_cap * a.c.kv_heads;
     const CUtensorMap map = page_map(a.c);
     const int ctas = (int)std::min<int64_t>((small + KS_WARPS - 1) / KS_WARPS, (a.rows <= 8 ? 3 : 2) * sms);
     if (a.rows <= 8)
@@ -799,11 +574,6 @@ void launch(const AttnKArgs& a, cudaStream_t s) {
         launch_small<T, 2>(a, map, ctas, s);
     if (a.b.max_keys > PG_CHUNK) {
         launch_pdl(k_kv8_join<T>, dim3(small_rows(a.b), a.b.requests, a.c.kv_heads), dim3(KJ_WARPS * 32), 0, s, a);
-        note_launch();
-    }
-    if ((int64_t)a.b.max_new * a.b.group > PG_SMALL_ROWS) {
-        k_kv8_large<T><<<(unsigned)std::min<int64_t>(large, 4 * sms), KA_THREADS, 0, s>>>(a);
-        JV_CUDA(cudaGetLastError());
         note_launch();
     }
 }
@@ -857,10 +627,13 @@ int jv_kv8_attention(const jv_kv8_cache* cache, const jv_paged_batch* batch, int
         a.part_o = (float*)((char*)ws + w.o);
         a.part_ml = (float2*)((char*)ws + w.ml);
         a.rows = tile_rows(*batch);
+        a.large_o = (float*)((char*)ws + w.large_o);
+        a.large_ml = (float2*)((char*)ws + w.large_ml);
         if (type == T_F16)
             launch<__half>(a, (cudaStream_t)stream);
         else
             launch<__nv_bfloat16>(a, (cudaStream_t)stream);
+        if (a.v.large_cap > 0) launch_kv8_large(a, type, (cudaStream_t)stream);
     });
 }
 

@@ -1,0 +1,566 @@
+// kv8_attn_tc.cu — attention over the 8-bit paged cache for requests of many query rows (prompts and
+// their chunks), on the 5th-generation tensor cores. The mathematics is kv8_attn.cu's: integer keys and
+// values, their scales in the exponent and in the denominator.
+//
+// One CTA = one KV head x a pair of query tiles A and B of 128 rows (128 / group tokens x the group's heads),
+// which share every block of 128 keys; per tile and block
+//   S = Q K^T   tcgen05.mma kind::f16, M = N = K = 128, S in TMEM (fp32)
+//   w = 2^(e - M) as fp16 pairs, over S in TMEM (a row per thread, M moves only past 2^8)
+//   O += W V    W as the TMEM operand, V from shared memory (MN-major)
+// TMEM: O_A, O_B, S_A / W_A, S_B / W_B, 128 columns each. S(b + 1) of a tile follows its W V(b) in the tensor
+// pipe, so S(b) complete means O holds the blocks before b; while one tile's rows are in the softmax the
+// other's products run.
+// Warps 0-3 and 4-7: the softmax and output of tiles A and B. Warps 8-11: convert the cache's int8 to fp16
+// operands (K as b + 128 in subnormals, one byte permute; V signed), two stages of K and two of V, the next
+// block's bytes already in registers. Warps 12 and 13: issue tile A's and B's products. Registers are moved
+// from the last two warpgroups to the softmax (128 at launch: 184 + 184 + 104 + 40 = 4 x 128). Every wait is
+// bounded; on expiry the role records its site and stops.
+#include <atomic>
+
+#include <cuda_bf16.h>
+
+#include "paged.h"
+#include "tc_common.cuh"
+
+namespace jv {
+namespace {
+
+constexpr int KT_THREADS = 512;
+constexpr int KT_KEYS = 128;
+constexpr int KT_TILE = 128 * 128 * 2;  // one fp16 operand tile
+constexpr int KT_SLOTS = 4;             // blocks whose scales are kept
+constexpr int KT_SMEM = 6 * KT_TILE + KT_SLOTS * 128 + 256 + 1024;
+
+enum KtRole : int { KR_CONVERT_K = 0, KR_CONVERT_V = 1, KR_ISSUE = 2, KR_SOFTMAX = 3 };
+
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
+
+// A from TMEM.
+__device__ __forceinline__ void umma_ta(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+                 "r"(a), "l"(bd), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
+    return ok != 0;
+}
+__device__ __forceinline__ float lg2_approx(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct KtItem {
+    RequestRows rr;
+    int tt;               // tokens per tile
+    int t0[2], nt[2];     // first token (of the request's new ones) and tokens of each tile
+    int b0[2], b1[2];     // its blocks
+    int lo, hi;           // blocks of the CTA
+};
+
+// 16 int8 of one row (dimensions 16 j ..) as 32 bytes of fp16 into a [128][128] operand tile. Lanes 0-3 of a
+// row's eight store their even chunk first, lanes 4-7 their odd one, so that eight lanes meet eight chunks.
+template <bool SIGNED>
+__device__ __forceinline__ void convert16(uint32_t tile, int row, int j, uint4 raw) {
+    const uint32_t w[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};
+    uint32_t h[8];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t fill = SIGNED ? 0x64646464u : 0u;
+        h[2 * e] = __byte_perm(w[e], fill, 0x4140);
+        h[2 * e + 1] = __byte_perm(w[e], fill, 0x4342);
+        if (SIGNED) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const __half2 x = __hsub2(*(const __half2*)&h[2 * e + k], __floats2half2_rn(1152.f, 1152.f));
+                h[2 * e + k] = *(const uint32_t*)&x;
+            }
+        }
+    }
+    const bool flip = j >= 4;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int c = 2 * j + (flip ? 1 - k : k);
+        const uint32_t at = tile + tile_off(row, c);
+        const uint32_t x0 = flip == (k == 0) ? h[4] : h[0], x1 = flip == (k == 0) ? h[5] : h[1], x2 = flip == (k == 0) ? h[6] : h[2],
+                       x3 = flip == (k == 0) ? h[7] : h[3];
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(x0), "r"(x1), "r"(x2), "r"(x3) : "memory");
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
+    extern __shared__ uint8_t kt_raw[];
+    uint8_t* sm = kt_raw + ((1024u - (s_addr(kt_raw) & 1023u)) & 1023u);
+    const uint32_t Qs = s_addr(sm), Ks = Qs + 2 * KT_TILE, Vs = Qs + 4 * KT_TILE;
+    float4* scales = (float4*)(sm + 6 * KT_TILE);  // [slot][8]: ks, log2 vs, 1 / vs of 16 keys
+    uint64_t* bars = (uint64_t*)(sm + 6 * KT_TILE + KT_SLOTS * 128);
+    const uint32_t k_full = s_addr(bars), v_full = k_full + 16, k_empty = k_full + 32, v_empty = k_full + 48;
+    const uint32_t q_full = k_full + 64, s_full = k_full + 80, p_full = k_full + 96, o_done = k_full + 112;
+    uint32_t* tslot = (uint32_t*)(bars + 16);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    pdl_wait();
+    pdl_launch_dependents();
+    const int kvh_n = a.c.kv_heads, kvh = blockIdx.x % kvh_n, index = blockIdx.x / kvh_n;
+    if (index >= a.v.head[1]) return;
+    const int4 item = a.v.large_items[index];
+    const int group = a.b.group, splits = item.w & 255, place = item.w >> 8;
+    KtItem it;
+    if (!request_rows(a.b, item.x, it.rr)) return;
+    it.tt = PG_TILE / group;
+    const int total_blocks = (int)(((int64_t)it.rr.len + KT_KEYS - 1) / KT_KEYS);
+    const int per = splits > 0 ? (total_blocks + splits - 1) / splits : 0;
+    if (item.y < 0 || item.z < 0 || item.z >= splits || (splits > 1 && (place < 0 || place + item.z >= a.v.split_cap)) || (int64_t)item.y * 2 * it.tt >= it.rr.n_new) return;
+    const int s0 = min(item.z * per, total_blocks), s1 = min(s0 + per, total_blocks);
+    it.lo = 1 << 30, it.hi = 0;
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        it.t0[x] = item.y * 2 * it.tt + x * it.tt;
+        it.nt[x] = max(0, min(it.tt, it.rr.n_new - it.t0[x]));
+        const int first = it.rr.len - it.rr.n_new + it.t0[x], last = first + it.nt[x] - 1;
+        it.b1[x] = it.nt[x] > 0 && last >= 0 ? min(s1, last / KT_KEYS + 1) : 0;
+        it.b0[x] = max(s0, a.window > 0 ? max(0, first + 1 - a.window) / KT_KEYS : 0);
+        if (it.b0[x] >= it.b1[x]) it.b0[x] = it.b1[x] = 0;
+        if (it.b0[x] < it.b1[x]) it.lo = min(it.lo, it.b0[x]), it.hi = max(it.hi, it.b1[x]);
+    }
+    if (it.lo > it.hi) it.lo = it.hi;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(k_full + 8 * i, 4);
+            mbar_init(v_full + 8 * i, 4);
+            mbar_init(k_empty + 8 * i, 2);
+            mbar_init(v_empty + 8 * i, 2);
+            mbar_init(q_full + 8 * i, 4);
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_full + 8 * i, 4);
+            mbar_init(o_done + 8 * i, 1);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 12) tmem_alloc(s_addr(tslot), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tslot;
+    int* err = a.b.status;
+
+    if (warp >= 12) {
+        reg_dec<40>();
+        if (warp < 14) {
+            // ------------------------------------------------ issue the products of one tile
+            const int x = warp - 12;
+            const uint32_t id_s = idesc_f16(KT_KEYS, PG_TILE), id_o = idesc_f16(PG_DIM, PG_TILE) | (1u << 16);
+            const uint32_t q = Qs + x * KT_TILE, o = tmem + (uint32_t)(x * 128), d = tmem + 256u + (uint32_t)(x * 128);
+            bool ok = true;
+            if (it.b0[x] < it.b1[x]) ok = warp_wait(q_full + 8 * x, 0);
+            for (int b = it.lo, n = 0; b < it.hi && ok; b++, n++) {
+                const uint32_t st = n & 1, ph = (n >> 1) & 1;
+                const bool mine = b >= it.b0[x] && b < it.b1[x];
+                const uint32_t k = Ks + st * KT_TILE, v = Vs + st * KT_TILE;
+                ok = __all_sync(0xffffffffu, mbar_poll(k_full + 8 * st, ph));
+                if (!ok) break;
+                if (mine) {
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < 8; kk++) {
+                            const uint32_t off = (uint32_t)((kk >> 2) * 16384 + (kk & 3) * 32);
+                            umma(d, sdesc(q + off), sdesc(k + off), id_s, kk > 0 ? 1u : 0u);
+                        }
+                        umma_commit(s_full + 8 * x);
+                        umma_commit(k_empty + 8 * st);
+                    }
+                    __syncwarp();
+                    ok = __all_sync(0xffffffffu, mbar_poll(p_full + 8 * x, (uint32_t)((b - it.b0[x]) & 1)));
+                    ok = ok && __all_sync(0xffffffffu, mbar_poll(v_full + 8 * st, ph));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < 8; kk++)
+                            umma_ta(o, d + (uint32_t)(8 * kk), sdesc_mn(v + kk * 2048), id_o, b > it.b0[x] || kk > 0 ? 1u : 0u);
+                        umma_commit(v_empty + 8 * st);
+                        if (b + 1 == it.b1[x]) umma_commit(o_done + 8 * x);
+                    }
+                    __syncwarp();
+                } else {
+                    // the other tile's block: released at once, but not before it is there (a release counts for
+                    // the stage's current use)
+                    ok = __all_sync(0xffffffffu, mbar_poll(v_full + 8 * st, ph));
+                    if (ok && lane == 0) {
+                        mbar_arrive(k_empty + 8 * st);
+                        mbar_arrive(v_empty + 8 * st);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (!ok && lane == 0) paged_report(err, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_TC + KR_ISSUE);
+        }
+    } else if (warp >= 8) {
+        reg_dec<104>();
+        // ---------------------------------------------------- int8 -> fp16 operands
+        const int t = tid - 256, j = t & 7, r0 = t >> 3;  // 16 bytes j of rows r0 + 16 k
+        const int32_t* table = a.b.block_table + (int64_t)item.x * a.b.max_blocks;
+        const int pages = (int)(((int64_t)it.rr.len + PG_TOKENS - 1) / PG_TOKENS);
+        // the two pages of a block; -1 where the request has none
+        auto page_of = [&](int b, int h) {
+            const int p = 2 * b + h;
+            if (b >= it.hi || p >= pages) return -1;
+            const int id = table[p];
+            if ((unsigned)id >= (unsigned)a.c.pages) {
+                if (t == 0) paged_report(err, JV_ERR_RANGE, PS_ATTN_PAGE);
+                return -1;
+            }
+            return id;
+        };
+        uint4 kr[8], vr[8];
+        auto load = [&](uint4 (&r)[8], int p0, int p1, int plane) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int id = k < 4 ? p0 : p1;
+                r[k] = make_uint4(0, 0, 0, 0);
+                if (id >= 0)
+                    r[k] = *(const uint4*)((const char*)a.c.data + (int64_t)id * a.c.page_bytes + (int64_t)(2 * kvh + plane) * PG_PLANE +
+                                           (r0 + 16 * (k & 3)) * PG_DIM + 16 * j);
+            }
+        };
+        int p0 = page_of(it.lo, 0), p1 = page_of(it.lo, 1);
+        int n0 = page_of(it.lo + 1, 0), n1 = page_of(it.lo + 1, 1);
+        load(kr, p0, p1, 0);
+        load(vr, p0, p1, 1);
+        bool ok = true;
+        for (int b = it.lo, n = 0; b < it.hi; b++, n++) {
+            const uint32_t st = n & 1, ph = ((n >> 1) & 1) ^ 1;
+            float4 sc = make_float4(0.f, 0.f, 1.f, 0.f);  // without a page nothing is visible
+            if (t < 8) {
+                const int id = t < 4 ? p0 : p1;
+                const int64_t key = (int64_t)b * KT_KEYS + t * PG_BLOCK;
+                if (id >= 0 && key < it.rr.len) {
+                    const float* s = a.c.scales + (int64_t)id * a.c.scale_stride + kvh * 8 + (t & 3);
+                    const float vs = s[4] > 0.f ? s[4] : 1.f;  // a block of zeros
+                    sc = make_float4(s[0], lg2_approx(vs), __frcp_rn(vs), 0.f);
+                }
+            }
+            ok = warp_wait(k_empty + 8 * st, ph);
+            if (!ok) {
+                if (lane == 0) paged_report(err, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_TC + KR_CONVERT_K);
+                break;
+            }
+            if (t < 8) scales[(n & (KT_SLOTS - 1)) * 8 + t] = sc;
+#pragma unroll
+            for (int k = 0; k < 8; k++) convert16<false>(Ks + st * KT_TILE, r0 + 16 * k, j, kr[k]);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(k_full + 8 * st);
+            load(kr, n0, n1, 0);
+            ok = warp_wait(v_empty + 8 * st, ph);
+            if (!ok) {
+                if (lane == 0) paged_report(err, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_TC + KR_CONVERT_V);
+                break;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) convert16<true>(Vs + st * KT_TILE, r0 + 16 * k, j, vr[k]);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(v_full + 8 * st);
+            load(vr, n0, n1, 1);
+            p0 = n0, p1 = n1;
+            n0 = page_of(b + 2, 0), n1 = page_of(b + 2, 1);
+        }
+    } else {
+        reg_inc<184>();
+        // ---------------------------------------------------- softmax and output, a query row per thread
+        const int x = warp >> 2, r = tid & 127;
+        const int tok = r / group, j = r - tok * group;
+        const bool live = tok < it.nt[x];
+        const int pos = it.rr.len - it.rr.n_new + it.t0[x] + tok;
+        // rows of no token see everything: they are not stored, and must not send their warp down the masked path
+        const int hi_key = live ? pos + 1 : 1 << 30, lo_key = live && a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+        const int64_t token = it.rr.start + it.t0[x] + tok;
+        const int head = kvh * group + j;
+        float qs = 0.f, qb = 0.f;
+        if (it.b0[x] < it.b1[x]) {
+            // the row to shared memory as fp16 (bf16: times a power of two, as in kv8_attn.cu), and its sum
+            uint32_t w[64];
+#pragma unroll
+            for (int c = 0; c < 16; c++) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (live) v = *(const uint4*)((const T*)a.q.in + token * a.q.in_token + (int64_t)head * a.q.in_head + 8 * c);
+                w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
+            }
+            float f = 1.f;
+            if (std::is_same<T, __nv_bfloat16>::value) {
+                float amax = 0.f;
+#pragma unroll
+                for (int e = 0; e < 64; e++)
+                    amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xffff0000u))));
+                const int ex = min(max((int)((__float_as_uint(amax) >> 23) & 0xff), 14), 254);
+                const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
+                f = 1.f / up;
+#pragma unroll
+                for (int e = 0; e < 64; e++) {
+                    const __half2 h = __floats2half2_rn(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xffff0000u) * up);
+                    w[e] = *(const uint32_t*)&h;
+                }
+            }
+            // a negative scale is taken into the row, so that the keys' factors below are never negative
+            f *= fabsf(a.scale);
+            const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 64; e++) {
+                w[e] ^= sign;
+                const float2 h = __half22float2(*(const __half2*)&w[e]);
+                sum += h.x + h.y;
+            }
+            qs = f * 16777216.f;  // K is there as (b + 128) 2^-24
+            qb = -128.f * sum * f;
+#pragma unroll
+            for (int c = 0; c < 16; c++)
+                *(uint4*)(sm + x * KT_TILE + tile_off(r, c)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full + 8 * x);
+        }
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t o_col = tmem + lanes + (uint32_t)(x * 128), s_col = tmem + lanes + 256u + (uint32_t)(x * 128);
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int b = it.b0[x]; b < it.b1[x]; b++) {
+            if (!warp_wait(s_full + 8 * x, (uint32_t)((b - it.b0[x]) & 1))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const float4* sc = scales + ((b - it.lo) & (KT_SLOTS - 1)) * 8;
+            uint32_t v[128];
+            {
+                uint32_t(&v0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[0]);
+                uint32_t(&v1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[32]);
+                uint32_t(&v2)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[64]);
+                uint32_t(&v3)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[96]);
+                tld32(s_col, v0);
+                tld32(s_col + 32u, v1);
+                tld32(s_col + 64u, v2);
+                tld32(s_col + 96u, v3);
+                tld_wait(v0);
+                tld_wait(v1);
+                tld_wait(v2);
+                tld_wait(v3);
+            }
+            const int k0 = b * KT_KEYS, vis_hi = hi_key - k0, vis_lo = lo_key - k0;
+            const bool all = __all_sync(0xffffffffu, vis_hi >= KT_KEYS && vis_lo <= 0);
+            float bm = -INFINITY;
+            if (!all) {
+                // a block that some row does not see whole: the exponents themselves, masked, in place
+#pragma unroll
+                for (int h = 0; h < 8; h++) {
+                    const float4 s = sc[h];
+                    const float ka = s.x * qs, kb = fmaf(s.x, qb, s.y);
+#pragma unroll
+                    for (int e = 16 * h; e < 16 * h + 16; e++) {
+                        const float y = fmaf(__uint_as_float(v[e]), ka, kb);
+                        v[e] = __float_as_uint(e < vis_hi && e >= vis_lo ? y : -INFINITY);
+                        bm = fmaxf(bm, __uint_as_float(v[e]));
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 8; h++) {
+                    const float4 s = sc[h];
+                    float g = __uint_as_float(v[16 * h]);
+#pragma unroll
+                    for (int e = 16 * h + 1; e < 16 * h + 16; e++) g = fmaxf(g, __uint_as_float(v[e]));
+                    bm = fmaxf(bm, fmaf(g, s.x * qs, fmaf(s.x, qb, s.y)));
+                }
+            }
+            const bool move = bm > m + 8.f;
+            const float mn = move ? bm : m;
+            const float ref = mn == -INFINITY ? 0.f : mn;
+            const float alpha = !move ? 1.f : m == -INFINITY ? 0.f : ex2(m - mn);
+            float rs = 0.f;
+#pragma unroll
+            for (int h = 0; h < 8; h++) {
+                const float4 s = sc[h];
+                const float ka = all ? s.x * qs : 1.f, kb = (all ? fmaf(s.x, qb, s.y) : 0.f) - ref;
+                float g = 0.f;
+#pragma unroll
+                for (int e = 16 * h; e < 16 * h + 16; e += 2) {
+                    const float w0 = ex2(fmaf(__uint_as_float(v[e]), ka, kb)), w1 = ex2(fmaf(__uint_as_float(v[e + 1]), ka, kb));
+                    g += w0 + w1;
+                    const __half2 hp = __floats2half2_rn(w0, w1);
+                    v[e >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
+                }
+                rs = fmaf(g, s.z, rs);
+            }
+            l = fmaf(l, alpha, rs);
+            m = mn;
+            tst32(s_col, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+            tst32(s_col + 32u, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+            // O *= alpha where a row's reference moved (S(b) complete: so is W V(b - 1))
+            if (b > it.b0[x] && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+                for (int h = 0; h < 4; h++) {
+                    uint32_t o[32];
+                    tld32(o_col + (uint32_t)(h * 32), o);
+                    tld_wait(o);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                    tst32(o_col + (uint32_t)(h * 32), o);
+                }
+            }
+            tst_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 8 * x);
+        }
+        const bool any = it.b0[x] < it.b1[x];
+        if (ok && any) ok = warp_wait(o_done + 8 * x, 0);
+        if (!ok) {
+            if (lane == 0) paged_report(err, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_TC + KR_SOFTMAX);
+        } else {
+            tc_fence_after();
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const int64_t part = ((int64_t)place * kvh_n + kvh) * 2 * PG_TILE + x * PG_TILE + r;
+#pragma unroll 1
+            for (int h = 0; h < 4; h++) {
+                uint32_t o[32];
+                if (any) {
+                    tld32(o_col + (uint32_t)(h * 32), o);
+                    tld_wait(o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0;
+                }
+                if (!live) continue;
+                if (splits == 1) {
+                    T* dst = (T*)a.q.out + token * a.q.out_token + (int64_t)head * a.q.out_head + 32 * h;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t y[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float y0 = __uint_as_float(o[8 * c + 2 * e]) * inv, y1 = __uint_as_float(o[8 * c + 2 * e + 1]) * inv;
+                            if (std::is_same<T, __half>::value) {
+                                const __half2 q = __floats2half2_rn(y0, y1);
+                                y[e] = *(const uint32_t*)&q;
+                            } else {
+                                const __nv_bfloat162 q = __floats2bfloat162_rn(y0, y1);
+                                y[e] = *(const uint32_t*)&q;
+                            }
+                        }
+                        *(uint4*)(dst + 8 * c) = make_uint4(y[0], y[1], y[2], y[3]);
+                    }
+                } else {
+                    float4* dst = (float4*)(a.large_o + part * PG_DIM + 32 * h);
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        dst[c] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
+                                             __uint_as_float(o[4 * c + 3]));
+                }
+            }
+            if (live && splits > 1) a.large_ml[part] = make_float2(m, l);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the splits of pairs of tiles: the grid's warps find the pairs that have some, 32 items a look, and
+// take a row each.
+constexpr int KTJ_WARPS = 8;
+template <class T>
+__device__ __forceinline__ void join_row(const AttnKArgs& a, int4 item, int kvh, int row, int lane) {
+    const int splits = item.w & 255, place = item.w >> 8;
+    RequestRows rr;
+    if (splits > 16 || place < 0 || place + splits > a.v.split_cap || !request_rows(a.b, item.x, rr)) return;
+    const int group = a.b.group, tt = PG_TILE / group, x = row / PG_TILE, r = row % PG_TILE, tok = r / group;
+    const int t = item.y * 2 * tt + x * tt + tok;
+    if (tok >= tt || t < 0 || t >= rr.n_new) return;
+    const int64_t p0 = ((int64_t)place * a.c.kv_heads + kvh) * 2 * PG_TILE + row, step = (int64_t)a.c.kv_heads * 2 * PG_TILE;
+    const float2 ml = lane < splits ? a.large_ml[p0 + lane * step] : make_float2(-INFINITY, 0.f);  // at most 16 splits
+    float m = ml.x;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float f = ex2(ml.x - (m == -INFINITY ? 0.f : m));
+    float l = ml.y * f;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < splits; s++) {
+        const float4 y = *(const float4*)(a.large_o + (p0 + s * step) * PG_DIM + 4 * lane);
+        const float g = __shfl_sync(0xffffffffu, f, s);
+        o.x = fmaf(y.x, g, o.x), o.y = fmaf(y.y, g, o.y), o.z = fmaf(y.z, g, o.z), o.w = fmaf(y.w, g, o.w);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* dst = (T*)a.q.out + (int64_t)(rr.start + t) * a.q.out_token + (int64_t)(kvh * group + r - tok * group) * a.q.out_head + 4 * lane;
+    if (std::is_same<T, __half>::value) {
+        const __half2 u = __floats2half2_rn(o.x * inv, o.y * inv), v = __floats2half2_rn(o.z * inv, o.w * inv);
+        *(uint2*)dst = make_uint2(*(const uint32_t*)&u, *(const uint32_t*)&v);
+    } else {
+        const __nv_bfloat162 u = __floats2bfloat162_rn(o.x * inv, o.y * inv), v = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+        *(uint2*)dst = make_uint2(*(const uint32_t*)&u, *(const uint32_t*)&v);
+    }
+}
+template <class T>
+__global__ void __launch_bounds__(KTJ_WARPS * 32) k_kv8_large_join(AttnKArgs a) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = blockIdx.x * KTJ_WARPS + (threadIdx.x >> 5), warps = gridDim.x * KTJ_WARPS;
+    const int n = (int)min((int64_t)a.v.head[1], a.v.large_cap);
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int4 mine = i0 + lane < n ? a.v.large_items[i0 + lane] : make_int4(0, 0, 1, 0);
+        uint32_t some = __ballot_sync(0xffffffffu, mine.z == 0 && (mine.w & 255) > 1);
+        for (; some; some &= some - 1) {
+            const int src = __ffs(some) - 1;
+            const int4 item = make_int4(__shfl_sync(0xffffffffu, mine.x, src), __shfl_sync(0xffffffffu, mine.y, src),
+                                        __shfl_sync(0xffffffffu, mine.z, src), __shfl_sync(0xffffffffu, mine.w, src));
+            for (int u = warp; u < a.c.kv_heads * 2 * PG_TILE; u += warps) join_row<T>(a, item, u / (2 * PG_TILE), u % (2 * PG_TILE), lane);
+        }
+    }
+}
+
+template <class T>
+void launch_large(const AttnKArgs& a, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    JV_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (!(done.load() & bit)) {
+        JV_CUDA(cudaFuncSetAttribute(k_kv8_large<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, KT_SMEM));
+        // the softmax's registers come out of what the launch was given: a build with fewer would wait for them for good
+        cudaFuncAttributes at;
+        JV_CUDA(cudaFuncGetAttributes(&at, k_kv8_large<T>));
+        if (at.numRegs != 128) throw Error(JV_ERR_DEVICE, "k_kv8_large was not built with 128 registers per thread");
+        done.fetch_or(bit);
+    }
+    const unsigned items = (unsigned)(a.v.large_cap * a.c.kv_heads);
+    launch_pdl(k_kv8_large<T>, dim3(items), dim3(KT_THREADS), KT_SMEM, s, a);
+    note_launch();
+    if (a.v.split_cap > 0 && a.b.max_blocks > 16) {  // a request of at most 1024 keys has no splits
+        launch_pdl(k_kv8_large_join<T>, dim3(2 * 148), dim3(KTJ_WARPS * 32), 0, s, a);
+        note_launch();
+    }
+}
+
+}  // namespace
+
+void launch_kv8_large(const AttnKArgs& a, int type, cudaStream_t s) {
+    if (type == T_F16)
+        launch_large<__half>(a, s);
+    else
+        launch_large<__nv_bfloat16>(a, s);
+}
+
+}  // namespace jv

@@ -86,7 +86,10 @@ PlanView plan_view(const jv_paged_batch& b) {
     const int64_t most = (int64_t)b.max_blocks * PG_TOKENS;  // of one request's keys
     const int64_t per = most <= 4096 ? std::min<int64_t>(32, (most + PG_CHUNK - 1) / PG_CHUNK) : std::max<int64_t>(512, (most + 2047) / 2048);
     v.small_cap = std::min(R + std::min(b.max_keys / PG_CHUNK, 32 * R + b.max_keys / 128), R * per) * tiles;
-    v.large_cap = std::min<int64_t>(R, T * b.group / (PG_SMALL_ROWS + 1)) + T * b.group / PG_TILE_ROWS;
+    const int64_t large = (int64_t)b.max_new * b.group > PG_SMALL_ROWS ? std::min<int64_t>(R, T * b.group / (PG_SMALL_ROWS + 1)) : 0;
+    // at most 16 / pairs splits of each of up to 7 pairs, and a split has at least 1024 keys but for a request's last
+    v.split_cap = std::min(16 * large, 7 * (large + b.max_keys / 1024));
+    v.large_cap = large ? v.split_cap + large + T / pg_pair_tokens(b.group) : 0;
     v.unit_cap = std::min<int64_t>(T, T / PG_BLOCK + 2 * R);
     uint8_t* p = (uint8_t*)b.work;
     int64_t at = 0;
@@ -97,7 +100,7 @@ PlanView plan_view(const jv_paged_batch& b) {
     };
     v.head = (int32_t*)take(8 * 4);
     v.first = (int32_t*)take(R * 4);
-    v.prefix = (int32_t*)take(3 * R * 4);
+    v.prefix = (int32_t*)take(4 * R * 4);
     v.small_items = (int4*)take(v.small_cap * 32);
     v.large_items = (int4*)take(v.large_cap * 16);
     v.units = (int2*)take(v.unit_cap * 8);
@@ -124,7 +127,7 @@ constexpr int PLAN_FILL_REQUESTS = 256;  // most requests that the first launch 
 
 // A request's place in the batch: its lengths and the exclusive sums in front of it.
 struct Place {
-    int old, n_new, start, page, unit, small, large;
+    int old, n_new, start, page, unit, small, large, split;  // split: large items with more than one split
 };
 
 __device__ __forceinline__ int units_of(int old, int n_new) {
@@ -137,8 +140,8 @@ __device__ __forceinline__ bool is_small(int n_new, int group) { return (int64_t
 __device__ __forceinline__ int small_of(int old, int n_new, int group) {
     return n_new > 0 && is_small(n_new, group) ? pg_chunks(old + n_new) * ((n_new * group + PG_ROW_TILE - 1) / PG_ROW_TILE) : 0;
 }
-__device__ __forceinline__ int large_of(int n_new, int group) {
-    return n_new > 0 && !is_small(n_new, group) ? (n_new * group + PG_TILE_ROWS - 1) / PG_TILE_ROWS : 0;
+__device__ __forceinline__ int large_of(int old, int n_new, int group) {
+    return n_new > 0 && !is_small(n_new, group) ? pg_pairs(n_new, group) * pg_splits(old + n_new, pg_pairs(n_new, group)) : 0;
 }
 
 // One request's pages, tokens, units and items, by threads t, t + n, ...
@@ -162,23 +165,25 @@ __device__ __forceinline__ void plan_request(const PlanArgs& a, int r, const Pla
         a.v.small_items[2 * (q.small + i)] = make_int4(r, i % chunks, chunks, i / chunks);
         a.v.small_items[2 * (q.small + i) + 1] = make_int4(q.start, q.n_new, q.old + q.n_new, 0);
     }
-    const int large = large_of(q.n_new, b.group);
-    // a request's last tile sees the most keys: first
-    for (int i = t; i < large; i += n) a.v.large_items[q.large + i] = make_int4(r, large - 1 - i, 0, 0);
+    const int large = large_of(q.old, q.n_new, b.group), pairs = pg_pairs(q.n_new, b.group);
+    const int splits = large > 0 ? large / pairs : 1;
+    // a request's last tiles see the most keys: first
+    for (int i = t; i < large; i += n)
+        a.v.large_items[q.large + i] = make_int4(r, pairs - 1 - i / splits, i % splits, splits | (splits > 1 ? (q.split + i) << 8 : 0));
 }
 
 // One CTA: the sums over the requests and the checks; with `fill`, everything else too, a warp per
 // request. Latency-bound: each thread holds up to 4 consecutive requests, the sums are one pass of
 // warp shuffles and one barrier (every warp adds up the warps' totals for itself).
 __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
-    __shared__ int ws[32][5];
+    __shared__ int ws[32][6];
     __shared__ long long wl[32][2];
     __shared__ Place places[PLAN_FILL_REQUESTS];
     const jv_paged_batch& b = a.b;
     const int R = b.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
     const int per = (R + blockDim.x - 1) / blockDim.x, r0 = tid * per;  // per <= PLAN_PER
     const int n_free = *a.n_free;
-    int old[PLAN_PER], n_new[PLAN_PER], sum[5] = {0, 0, 0, 0, 0};
+    int old[PLAN_PER], n_new[PLAN_PER], sum[6] = {0, 0, 0, 0, 0, 0};
     long long keys = 0, tokens = 0;
     bool bad = false;
 #pragma unroll
@@ -200,11 +205,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
         sum[1] += pages_of(old[j], n_new[j]);
         sum[2] += units_of(old[j], n_new[j]);
         sum[3] += small_of(old[j], n_new[j], b.group);
-        sum[4] += large_of(n_new[j], b.group);
+        const int large = large_of(old[j], n_new[j], b.group);
+        sum[4] += large;
+        sum[5] += large > pg_pairs(n_new[j], b.group) ? large : 0;
     }
-    int pre[5];
+    int pre[6];
 #pragma unroll
-    for (int k = 0; k < 5; k++) {
+    for (int k = 0; k < 6; k++) {
         int x = sum[k];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -221,11 +228,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
     }
     if (lane == 0) wl[warp][0] = keys, wl[warp][1] = tokens;
     bad = __syncthreads_or(bad);
-    int tot[5];
+    int tot[6];
     {
-        int before[5];
+        int before[6];
 #pragma unroll
-        for (int k = 0; k < 5; k++) {
+        for (int k = 0; k < 6; k++) {
             const int x = lane < warps ? ws[lane][k] : 0;
             before[k] = lane < warp ? x : 0;
             tot[k] = x;
@@ -235,7 +242,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) {
 #pragma unroll
-            for (int k = 0; k < 5; k++) {
+            for (int k = 0; k < 6; k++) {
                 before[k] += __shfl_xor_sync(0xffffffffu, before[k], o);
                 tot[k] += __shfl_xor_sync(0xffffffffu, tot[k], o);
             }
@@ -243,7 +250,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
             tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
         }
 #pragma unroll
-        for (int k = 0; k < 5; k++) pre[k] += before[k];
+        for (int k = 0; k < 6; k++) pre[k] += before[k];
     }
     int code = 0, site = 0;  // the same in every thread
     if (bad)
@@ -265,7 +272,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
     for (int j = 0; j < PLAN_PER; j++) {
         const int r = r0 + j;
         if (j >= per || r >= R) continue;
-        const Place q = {old[j], ok ? n_new[j] : 0, ok ? pre[0] : 0, ok ? pre[1] : 0, ok ? pre[2] : 0, ok ? pre[3] : 0, ok ? pre[4] : 0};
+        const Place q = {old[j], ok ? n_new[j] : 0, ok ? pre[0] : 0, ok ? pre[1] : 0, ok ? pre[2] : 0, ok ? pre[3] : 0, ok ? pre[4] : 0,
+                         ok ? pre[5] : 0};
         b.lengths[r] = q.old + q.n_new;
         b.starts[r] = q.start;
         a.v.first[r] = q.small;
@@ -275,12 +283,15 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
             prefix[r] = q.page;
             prefix[R + r] = q.unit;
             prefix[2 * R + r] = q.large;
+            prefix[3 * R + r] = q.split;
         }
         pre[0] += n_new[j];
         pre[1] += pages_of(old[j], n_new[j]);
         pre[2] += units_of(old[j], n_new[j]);
         pre[3] += small_of(old[j], n_new[j], b.group);
-        pre[4] += large_of(n_new[j], b.group);
+        const int large = large_of(old[j], n_new[j], b.group);
+        pre[4] += large;
+        pre[5] += large > pg_pairs(n_new[j], b.group) ? large : 0;
     }
     if (tid == 0) {
         b.starts[R] = ok ? tot[0] : 0;
@@ -304,7 +315,8 @@ __global__ void __launch_bounds__(PLAN_FILL_THREADS) k_plan_fill(PlanArgs a) {
     const jv_paged_batch& b = a.b;
     const int r = blockIdx.x, R = b.requests;
     const int len = b.lengths[r], start = b.starts[r], n_new = b.starts[r + 1] - start;
-    const Place q = {len - n_new, n_new, start, a.v.prefix[r], a.v.prefix[R + r], a.v.first[r], a.v.prefix[2 * R + r]};
+    const Place q = {len - n_new, n_new, start, a.v.prefix[r], a.v.prefix[R + r], a.v.first[r], a.v.prefix[2 * R + r],
+                     a.v.prefix[3 * R + r]};
     const int n_free = a.v.head[3];
     if (n_new > 0) plan_request(a, r, q, n_free, blockIdx.y * PLAN_FILL_THREADS + threadIdx.x, gridDim.y * PLAN_FILL_THREADS);
 }

@@ -14,11 +14,11 @@ constexpr int PG_MAX_REQUESTS = 4096;
 constexpr int PG_MAX_GROUP = 16;
 
 // A request whose new tokens x group give at most PG_SMALL_ROWS query rows is "small": its keys are
-// split into chunks that different CTAs take, PG_ROW_TILE rows at a time (kv8_attn.cu). The others go by
-// tiles of query rows over all their keys.
+// split into chunks that different warps take, PG_ROW_TILE rows at a time (kv8_attn.cu). The others go by
+// pairs of 128-row tiles to the tensor cores (kv8_attn_tc.cu).
 constexpr int PG_SMALL_ROWS = 32;
 constexpr int PG_ROW_TILE = 16;
-constexpr int PG_TILE_ROWS = 16;
+constexpr int PG_TILE = 128;  // query rows of a tensor-core tile; a large item is two tiles
 
 // Keys per chunk of a small request: 64 up to 2048 keys, where latency counts; then as many as keep what a
 // chunk leaves behind (rows x 528 bytes, written and read again) small against its keys. It goes by the
@@ -34,15 +34,25 @@ __host__ __device__ inline int pg_chunks(int len) {
     return len <= 0 ? 0 : (int)(((int64_t)len + pg_chunk_keys(len) - 1) / pg_chunk_keys(len));
 }
 
+// Tokens of a large item (two tiles of 128 / group tokens), and the items of a request: its keys are split
+// too, in up to 16 parts of at least 1024 keys, where it has few tiles. By the request's own sizes again.
+__host__ __device__ inline int pg_pair_tokens(int group) { return 2 * (PG_TILE / group); }
+__host__ __device__ inline int pg_pairs(int n_new, int group) { return (n_new + pg_pair_tokens(group) - 1) / pg_pair_tokens(group); }
+__host__ __device__ inline int pg_splits(int len, int pairs) {
+    if (pairs >= 8) return 1;
+    const int blocks = (int)(((int64_t)len + 127) / 128), most = (blocks + 7) / 8;
+    return most < 1 ? 1 : most < 16 / pairs ? most : 16 / pairs;
+}
+
 // A plan's work lists, in jv_paged_batch.work.
 struct PlanView {
     int32_t* head;      // [8]: small items, large items, append units, free pages before the step
     int32_t* first;     // [requests] first small item of each request
-    int32_t* prefix;    // [3][requests]: pages taken, units and large items before request r
+    int32_t* prefix;    // [4][requests]: pages taken, units, large items and those with splits before request r
     int4* small_items;  // two each: {request, chunk, chunks, row tile}, {start, new, length, 0}; row tile by row tile
-    int4* large_items;  // {request, tile, 0, 0}
+    int4* large_items;  // {request, pair of tiles, split, splits + 256 x place of its partials}; a pair's splits next to each other
     int2* units;        // {request, block}: the 16-token blocks the step writes to
-    int64_t small_cap, large_cap, unit_cap, bytes;
+    int64_t small_cap, large_cap, split_cap, unit_cap, bytes;  // split_cap: most large items with more than one split
 };
 PlanView plan_view(const jv_paged_batch& b);
 
@@ -77,8 +87,25 @@ int paged_api(F&& f) {
 enum PagedSite : int {
     PS_PLAN_LENGTH = 96, PS_PLAN_TOKENS = 97, PS_PLAN_KEYS = 98, PS_PLAN_FREE = 99, PS_PLAN_PAGE = 100,
     PS_APPEND_PAGE = 101, PS_APPEND_VALUE = 102, PS_READ_SLOT = 103, PS_READ_VALUE = 104, PS_ATTN_REQUEST = 105,
-    PS_ATTN_PAGE = 106, PS_ROPE_VALUE = 107, PS_ATTN_WAIT = 108
+    PS_ATTN_PAGE = 106, PS_ROPE_VALUE = 107, PS_ATTN_WAIT = 108, PS_ATTN_TC = 112 /* + role */
 };
+
+// An attention launch.
+struct AttnKArgs {
+    jv_kv8_cache c;
+    jv_paged_batch b;
+    PlanView v;
+    jv_heads q;
+    float scale;  // times log2 e
+    int window;
+    float* part_o;    // [small item][kv head][rows][128]
+    float2* part_ml;  // [small item][kv head][rows]
+    int rows;         // query rows of a small item's partials
+    float* large_o;   // [large item with splits][kv head][256][128]
+    float2* large_ml; // [large item with splits][kv head][256]
+};
+// Large requests, and the joining of their splits (kv8_attn_tc.cu).
+void launch_kv8_large(const AttnKArgs& a, int type, cudaStream_t s);
 
 #ifdef __CUDACC__
 __device__ __forceinline__ void paged_report(int32_t* status, int code, int site) {
