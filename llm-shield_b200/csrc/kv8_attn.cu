@@ -104,11 +104,26 @@ __device__ __forceinline__ void store_row(const AttnKArgs& a, int start, int kvh
 // next keys or already with the first of its next item. Nothing joins the warps: a chunk's result goes to
 // the workspace (k_kv8_join), or out when the request has one chunk. Bound by HBM: 12 warps keep 96 KB per SM
 // in flight; a 16-key tile costs about 250 instructions, a third of the issue slots at the HBM rate.
+// With two 8-row tiles per warp (NT = 2) the registers leave 8 warps per SM, with a third stage each. (Query
+// fragments in shared memory instead, for 12 warps: 108 against 88 us for 24 requests of 2 to 6 new tokens.)
 constexpr int KS_WARPS = 4;
-constexpr int KS_KEYS = 32;                        // keys per stage
-constexpr int KS_HALF = KS_KEYS * PG_DIM;          // bytes of K or V in a stage
-constexpr int KS_STAGES = 2;
-constexpr int KS_SMEM = KS_WARPS * KS_STAGES * 2 * KS_HALF + 1024;
+template <int NT>
+struct Ks {
+    static constexpr int keys = 32;                 // per stage
+    static constexpr int ctas = NT == 1 ? 3 : 2;    // per SM
+    static constexpr int stages = NT == 1 ? 2 : 3;
+    static constexpr int half = keys * PG_DIM;      // bytes of K or V in a stage
+    static constexpr int ring = stages * 2 * half;  // bytes of a warp's stages
+    static constexpr int smem = KS_WARPS * ring + 1024;
+};
+// A place in a warp's ring and the parity of its current use.
+template <int STAGES>
+struct Turn {
+    uint32_t stage = 0, parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++stage == STAGES) stage = 0, parity ^= 1;
+    }
+};
 
 __device__ __forceinline__ void tma_keys(uint32_t dst, const CUtensorMap* map, int row, int kvh, int page, uint32_t bar) {
     asm volatile(
@@ -125,14 +140,15 @@ struct KsItem {
 };
 
 template <class T, int NT>
-__global__ void __launch_bounds__(KS_WARPS * 32, NT == 1 ? 3 : 2) k_kv8_small(AttnKArgs a, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(KS_WARPS * 32, Ks<NT>::ctas) k_kv8_small(AttnKArgs a, const __grid_constant__ CUtensorMap map) {
+    constexpr int KEYS = Ks<NT>::keys, HALF = Ks<NT>::half, STAGES = Ks<NT>::stages, H = KEYS / PG_BLOCK;
     extern __shared__ uint8_t ks_raw[];
-    __shared__ uint64_t bars[KS_WARPS * KS_STAGES];
+    __shared__ uint64_t bars[KS_WARPS * STAGES];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, i = lane & 3;
-    uint8_t* sm = ks_raw + ((1024u - (s_addr(ks_raw) & 1023u)) & 1023u) + warp * KS_STAGES * 2 * KS_HALF;
-    const uint32_t base = s_addr(sm), full = s_addr(bars + warp * KS_STAGES);
+    uint8_t* sm = ks_raw + ((1024u - (s_addr(ks_raw) & 1023u)) & 1023u) + warp * Ks<NT>::ring;
+    const uint32_t base = s_addr(sm), full = s_addr(bars + warp * STAGES);
     if (lane == 0) {
-        for (int s = 0; s < KS_STAGES; s++) mbar_init(full + 8 * s, 1);
+        for (int s = 0; s < STAGES; s++) mbar_init(full + 8 * s, 1);
         fence_barrier_init();
     }
     __syncwarp();
@@ -171,32 +187,33 @@ __global__ void __launch_bounds__(KS_WARPS * 32, NT == 1 ? 3 : 2) k_kv8_small(At
         t.pages = t.page0 * PG_TOKENS + lane * PG_TOKENS < t.hi ? a.b.block_table[(int64_t)x.x * a.b.max_blocks + t.page0 + lane] : 0;
         return t;
     };
-    // Stage `n & 1` takes step t of an item (keys 32 t ..); a page that is not in the cache is not read.
-    auto issue = [&](const KsItem& it, int t, uint32_t n) {
-        const int page = __shfl_sync(0xffffffffu, it.pages, t * KS_KEYS / PG_TOKENS - it.page0);
+    // The stage of `turn` takes step t of an item (keys KEYS t ..); a page that is not in the cache is not read.
+    auto issue = [&](const KsItem& it, int t, Turn<STAGES>& turn) {
+        const int page = __shfl_sync(0xffffffffu, it.pages, t * KEYS / PG_TOKENS - it.page0);
         const bool there = (unsigned)page < (unsigned)a.c.pages;
         if (lane == 0) {
-            const uint32_t bar = full + 8 * (n & 1), dst = base + (n & 1) * 2 * KS_HALF;
-            mbar_expect_tx(bar, there ? 2 * KS_HALF : 0);
+            const uint32_t bar = full + 8 * turn.stage, dst = base + turn.stage * 2 * HALF;
+            mbar_expect_tx(bar, there ? 2 * HALF : 0);
             if (there) {
-                const int row = t * KS_KEYS % PG_TOKENS;
+                const int row = t * KEYS % PG_TOKENS;
                 tma_keys(dst, &map, row, it.kvh, page, bar);
-                tma_keys(dst + KS_HALF, &map, PG_TOKENS + row, it.kvh, page, bar);
+                tma_keys(dst + HALF, &map, PG_TOKENS + row, it.kvh, page, bar);
             } else {
                 paged_report(a.b.status, JV_ERR_RANGE, PS_ATTN_PAGE);
             }
         }
         __syncwarp();
+        turn.next();
     };
-    auto scales_of = [&](const KsItem& it, int t, float2& k, float2& v) {
-        const int page = __shfl_sync(0xffffffffu, it.pages, t * KS_KEYS / PG_TOKENS - it.page0);
-        k = v = make_float2(1.f, 1.f);
-        if ((unsigned)page < (unsigned)a.c.pages) {
-            const float* p = a.c.scales + (int64_t)page * a.c.scale_stride + it.kvh * 8 + t * KS_KEYS % PG_TOKENS / PG_BLOCK;
-            k = *(const float2*)p;
-            v = *(const float2*)(p + 4);
+    auto scales_of = [&](const KsItem& it, int t, float (&k)[H], float (&v)[H]) {
+        const int page = __shfl_sync(0xffffffffu, it.pages, t * KEYS / PG_TOKENS - it.page0);
+        const bool there = (unsigned)page < (unsigned)a.c.pages;
+        if (there) {
+            const float* p = a.c.scales + (int64_t)page * a.c.scale_stride + it.kvh * 8 + t * KEYS % PG_TOKENS / PG_BLOCK;
+#pragma unroll
+            for (int h = 0; h < H; h++) k[h] = p[h], v[h] = p[4 + h];
         }
-        return (unsigned)page < (unsigned)a.c.pages;
+        return there;
     };
 
     // Rows of a 16-key tile by fragment row: evens stay, odds are exchanged 4 apart, so that the lanes that load
@@ -210,25 +227,26 @@ __global__ void __launch_bounds__(KS_WARPS * 32, NT == 1 ? 3 : 2) k_kv8_small(At
     fetch(unit, px, py);
     KsItem cur = decode(unit, px, py);
     fetch(unit + stride, px, py);
-    uint32_t issued = 0, used = 0;  // stages over the warp's life
-    int at = cur.lo / KS_KEYS;      // next step of `cur` to issue
-    for (int s = 0; s < KS_STAGES && at * KS_KEYS < cur.hi; s++) issue(cur, at++, issued++);
+    Turn<STAGES> in, out;     // stages filled and used
+    int flight = 0;           // filled and not yet used
+    int at = cur.lo / KEYS;   // next step of `cur` to issue
+    for (; flight < STAGES && at * KEYS < cur.hi; flight++) issue(cur, at++, in);
     for (; unit < total; unit += stride) {
         const KsItem nxt = decode(unit + stride, px, py);
         fetch(unit + 2 * stride, px, py);
-        int nat = nxt.lo / KS_KEYS;
+        int nat = nxt.lo / KEYS;
         if (cur.valid) {
-            uint32_t qf[NT][16];
+            uint32_t qr[NT][16];
             float qs[NT][2], qb[NT][2], acc[NT][8][4], m[NT][2], l[NT][2];
-            int lo_key[NT][2], hi_key[NT][2];
             const int first = cur.len - cur.n_new + cur.row0 / group;
             const int last = cur.len - cur.n_new + (cur.row0 + cur.n_rows - 1) / group;
             const int all_hi = min(first + 1, cur.hi), all_lo = max(cur.lo, a.window > 0 ? last + 1 - a.window : 0);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const int row = 8 * n + g;
+                uint32_t qf[16];
 #pragma unroll
-                for (int e = 0; e < 16; e++) qf[n][e] = 0;
+                for (int e = 0; e < 16; e++) qf[e] = 0;
                 if (row < cur.n_rows) {
                     const int r = cur.row0 + row;
                     const T* src = (const T*)a.q.in + (int64_t)(cur.start + r / group) * a.q.in_token +
@@ -236,31 +254,32 @@ __global__ void __launch_bounds__(KS_WARPS * 32, NT == 1 ? 3 : 2) k_kv8_small(At
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const uint4 x = *(const uint4*)(src + 64 * (j >> 1) + 8 * (j & 1));
-                        qf[n][4 * j] = x.x, qf[n][4 * j + 1] = x.y, qf[n][4 * j + 2] = x.z, qf[n][4 * j + 3] = x.w;
+                        qf[4 * j] = x.x, qf[4 * j + 1] = x.y, qf[4 * j + 2] = x.z, qf[4 * j + 3] = x.w;
                     }
                 }
                 float f = 1.f;
-                if (std::is_same<T, __nv_bfloat16>::value) f = 1.f / q_to_f16(qf[n]);
+                if (std::is_same<T, __nv_bfloat16>::value) f = 1.f / q_to_f16(qf);
                 f *= a.scale;
                 // The K fragments are the bytes b + 128 as fp16 subnormals, (b + 128) 2^-24: an exact operand for
                 // one byte permute. q . kint = 2^24 (q . frag) - 128 sum q; the sum of the row is taken here.
                 float sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    const float2 x = __half22float2(*(const __half2*)&qf[n][e]);
+                    const float2 x = __half22float2(*(const __half2*)&qf[e]);
                     sum += x.x + x.y;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    qr[n][e] = qf[e];
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const int col = 2 * i + e, r = 8 * n + col;
+                    const int col = 2 * i + e;
                     qs[n][e] = __shfl_sync(0xffffffffu, f, 4 * col);
                     qb[n][e] = -128.f * __shfl_sync(0xffffffffu, sum, 4 * col) * qs[n][e];
                     qs[n][e] *= 16777216.f;
-                    const int pos = cur.len - cur.n_new + (cur.row0 + r) / group;
-                    hi_key[n][e] = r < cur.n_rows ? min(pos + 1, cur.hi) : 0;
-                    lo_key[n][e] = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
                     m[n][e] = -INFINITY;
                     l[n][e] = 0.f;
                 }
@@ -269,143 +288,155 @@ __global__ void __launch_bounds__(KS_WARPS * 32, NT == 1 ? 3 : 2) k_kv8_small(At
 #pragma unroll
                     for (int e = 0; e < 4; e++) acc[n][j][e] = 0.f;
             }
-            float2 ks, vs;
+            float ks[H], vs[H];
             bool there = false;
-            if (cur.lo < cur.hi) there = scales_of(cur, cur.lo / KS_KEYS, ks, vs);
-            for (int t = cur.lo / KS_KEYS; t * KS_KEYS < cur.hi; t++) {
-                const uint32_t st = used & 1;
-                if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, (used >> 1) & 1))) {
+            if (cur.lo < cur.hi) there = scales_of(cur, cur.lo / KEYS, ks, vs);
+            for (int t = cur.lo / KEYS; t * KEYS < cur.hi; t++) {
+                if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * out.stage, out.parity))) {
                     if (lane == 0) paged_report(a.b.status, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_WAIT);
-                    if (issued - used > 1) mbar_wait(full + 8 * (st ^ 1), ((used + 1) >> 1) & 1);  // a copy still in flight
+                    for (out.next(); --flight > 0; out.next()) mbar_wait(full + 8 * out.stage, out.parity);  // copies still in flight
                     return;
                 }
-                used++;
-                const float2 ks_t = ks;
-                float2 vs_t = vs;
+                float ks_t[H], vs_t[H];
                 const bool there_t = there;
-                if ((t + 1) * KS_KEYS < cur.hi) there = scales_of(cur, t + 1, ks, vs);
-                const int key0 = t * KS_KEYS;
+                const int key0 = t * KEYS;
+#pragma unroll
+                for (int h = 0; h < H; h++) {
+                    ks_t[h] = ks[h];
+                    // a block of zeros, or one without a key of the request
+                    vs_t[h] = vs[h] > 0.f && key0 + h * PG_BLOCK < cur.hi ? vs[h] : 1.f;
+                }
+                if ((t + 1) * KEYS < cur.hi) there = scales_of(cur, t + 1, ks, vs);
                 if (there_t) {
-                    const uint8_t* kp = sm + st * 2 * KS_HALF;
-                    const bool second = key0 + PG_BLOCK < cur.hi;  // the second tile has a key of the request
-                    if (!(vs_t.x > 0.f)) vs_t.x = 1.f;  // a block of zeros
-                    if (!second || !(vs_t.y > 0.f)) vs_t.y = 1.f;
-                    float s[2][NT][4];
+                    const bool all = key0 >= all_lo && key0 + KEYS <= all_hi;
+                    {
+                        const uint8_t* kp = sm + out.stage * 2 * HALF;
+                        float s[H][NT][4];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint4 kr[2][2];
+                        for (int h = 0; h < H; h++) {
+                            uint4 kr[2][2];
 #pragma unroll
-                        for (int r = 0; r < 2; r++) {
-                            kr[r][0] = *(const uint4*)(kp + h * PG_BLOCK * PG_DIM + 8 * r * PG_DIM + k_off + k_c0);
-                            kr[r][1] = *(const uint4*)(kp + h * PG_BLOCK * PG_DIM + 8 * r * PG_DIM + k_off + k_c1);
-                        }
+                            for (int r = 0; r < 2; r++) {
+                                kr[r][0] = *(const uint4*)(kp + h * PG_BLOCK * PG_DIM + 8 * r * PG_DIM + k_off + k_c0);
+                                kr[r][1] = *(const uint4*)(kp + h * PG_BLOCK * PG_DIM + 8 * r * PG_DIM + k_off + k_c1);
+                            }
 #pragma unroll
-                        for (int n = 0; n < NT; n++)
+                            for (int n = 0; n < NT; n++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) s[h][n][e] = 0.f;
+                                for (int e = 0; e < 4; e++) s[h][n][e] = 0.f;
 #pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const uint32_t w0[4] = {kr[0][j].x, kr[0][j].y, kr[0][j].z, kr[0][j].w};
-                            const uint32_t w1[4] = {kr[1][j].x, kr[1][j].y, kr[1][j].z, kr[1][j].w};
+                            for (int j = 0; j < 2; j++) {
+                                const uint32_t w0[4] = {kr[0][j].x, kr[0][j].y, kr[0][j].z, kr[0][j].w};
+                                const uint32_t w1[4] = {kr[1][j].x, kr[1][j].y, kr[1][j].z, kr[1][j].w};
 #pragma unroll
-                            for (int w = 0; w < 4; w++) {
-                                const uint32_t x0 = w0[w] ^ 0x80808080u, x1 = w1[w] ^ 0x80808080u;
-                                const uint32_t f[4] = {__byte_perm(x0, 0, 0x4140), __byte_perm(x1, 0, 0x4140), __byte_perm(x0, 0, 0x4342),
-                                                       __byte_perm(x1, 0, 0x4342)};
+                                for (int w = 0; w < 4; w++) {
+                                    const uint32_t x0 = w0[w] ^ 0x80808080u, x1 = w1[w] ^ 0x80808080u;
+                                    const uint32_t f[4] = {__byte_perm(x0, 0, 0x4140), __byte_perm(x1, 0, 0x4140),
+                                                           __byte_perm(x0, 0, 0x4342), __byte_perm(x1, 0, 0x4342)};
 #pragma unroll
-                                for (int n = 0; n < NT; n++) mma_f16(s[h][n], f, qf[n][8 * j + 2 * w], qf[n][8 * j + 2 * w + 1]);
+                                    for (int n = 0; n < NT; n++) mma_f16(s[h][n], f, qr[n][8 * j + 2 * w], qr[n][8 * j + 2 * w + 1]);
+                                }
                             }
                         }
-                    }
-                    const bool all = key0 >= all_lo && key0 + KS_KEYS <= all_hi;
-                    const float lv[2] = {lg2f(vs_t.x), lg2f(vs_t.y)}, iv[2] = {__frcp_rn(vs_t.x), __frcp_rn(vs_t.y)};
-                    const float kk[2] = {ks_t.x, ks_t.y};
-                    uint32_t pb[2][NT][2];
+                        uint32_t pb[H][NT][2];
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        float e[2][4], mx[2];
+                        for (int n = 0; n < NT; n++) {
+                            float e[H][4], mx[2], iv[H];
 #pragma unroll
-                        for (int h = 0; h < 2; h++)
+                            for (int h = 0; h < H; h++) {
+                                const float kk = ks_t[h], lv = lg2f(vs_t[h]);
+                                iv[h] = __frcp_rn(vs_t[h]);
+#pragma unroll
+                                for (int c = 0; c < 2; c++) {
+                                    const float ka = kk * qs[n][c], kb = fmaf(kk, qb[n][c], lv);
+                                    e[h][c] = fmaf(s[h][n][c], ka, kb);
+                                    e[h][c + 2] = fmaf(s[h][n][c + 2], ka, kb);
+                                }
+                            }
+                            if (!all) {
+#pragma unroll
+                                for (int c = 0; c < 2; c++) {
+                                    const int r = 8 * n + 2 * i + c, pos = cur.len - cur.n_new + (cur.row0 + r) / group;
+                                    const int hi_key = r < cur.n_rows ? min(pos + 1, cur.hi) : 0, lo_key = a.window > 0 ? pos + 1 - a.window : 0;
+#pragma unroll
+                                    for (int h = 0; h < H; h++)
+#pragma unroll
+                                        for (int x = c; x < 4; x += 2) {
+                                            const int key = key0 + h * PG_BLOCK + krow + 8 * (x >> 1);
+                                            if (key >= hi_key || key < lo_key) e[h][x] = -INFINITY;
+                                        }
+                                }
+                            }
+                            bool move = false;
 #pragma unroll
                             for (int c = 0; c < 2; c++) {
-                                const float ka = kk[h] * qs[n][c], kb = fmaf(kk[h], qb[n][c], lv[h]);
-                                e[h][c] = fmaf(s[h][n][c], ka, kb);
-                                e[h][c + 2] = fmaf(s[h][n][c + 2], ka, kb);
+                                mx[c] = fmaxf(e[0][c], e[0][c + 2]);
+                                if (H == 2) mx[c] = fmaxf(mx[c], fmaxf(e[H - 1][c], e[H - 1][c + 2]));
+                                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
+                                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 8));
+                                mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 16));
+                                move |= mx[c] > m[n][c] + 8.f;
                             }
-                        if (!all) {
+                            // the reference moves only when a score passes it by 2^8 (weights stay below 2^8)
+                            if (__any_sync(0xffffffffu, move)) {
+                                float alpha[2];
 #pragma unroll
-                            for (int h = 0; h < 2; h++)
+                                for (int c = 0; c < 2; c++) {
+                                    const float mn = fmaxf(m[n][c], mx[c]);
+                                    alpha[c] = m[n][c] == -INFINITY ? 0.f : ex2(m[n][c] - mn);
+                                    m[n][c] = mn;
+                                    l[n][c] *= alpha[c];
+                                }
 #pragma unroll
-                                for (int x = 0; x < 4; x++) {
-                                    const int key = key0 + h * PG_BLOCK + krow + 8 * (x >> 1);
-                                    if (key >= hi_key[n][x & 1] || key < lo_key[n][x & 1]) e[h][x] = -INFINITY;
+                                for (int j = 0; j < 8; j++)
+#pragma unroll
+                                    for (int x = 0; x < 4; x++) acc[n][j][x] *= alpha[x & 1];
+                            }
+#pragma unroll
+                            for (int h = 0; h < H; h++) {
+#pragma unroll
+                                for (int c = 0; c < 2; c++) {
+                                    const float ref = m[n][c] == -INFINITY ? 0.f : m[n][c];
+                                    e[h][c] = ex2(e[h][c] - ref);
+                                    e[h][c + 2] = ex2(e[h][c + 2] - ref);
+                                    l[n][c] = fmaf(e[h][c] + e[h][c + 2], iv[h], l[n][c]);
+                                }
+                                pb[h][n][0] = movmatrix_trans(pack2<__half>(e[h][0], e[h][1]));
+                                pb[h][n][1] = movmatrix_trans(pack2<__half>(e[h][2], e[h][3]));
+                            }
+                        }
+                        // O^T += V^T P^T: dimension 16 g + 2 j is the tile's row g, 16 g + 2 j + 1 its row g + 8. The
+                        // V fragments are signed integers (1024 + b + 128 - 1152): sums over thousands of keys would
+                        // lose what an offset left in them.
+#pragma unroll
+                        for (int h = 0; h < H; h++) {
+                            const uint8_t* vp = kp + HALF + h * PG_BLOCK * PG_DIM;
+                            const uint4 ra = *(const uint4*)(vp + v_off0), rb = *(const uint4*)(vp + v_off1);
+                            const uint4 rc = *(const uint4*)(vp + v_off0 + 8 * PG_DIM), rd = *(const uint4*)(vp + v_off1 + 8 * PG_DIM);
+                            const uint32_t va[4] = {ra.x, ra.y, ra.z, ra.w}, vb[4] = {rb.x, rb.y, rb.z, rb.w};
+                            const uint32_t vc[4] = {rc.x, rc.y, rc.z, rc.w}, vd[4] = {rd.x, rd.y, rd.z, rd.w};
+#pragma unroll
+                            for (int w = 0; w < 4; w++)
+#pragma unroll
+                                for (int u = 0; u < 2; u++) {
+                                    const uint32_t sel = u ? 0x7362 : 0x5140;
+                                    const uint32_t lo = __byte_perm(va[w], vb[w], sel) ^ 0x80808080u;
+                                    const uint32_t hi = __byte_perm(vc[w], vd[w], sel) ^ 0x80808080u;
+                                    const uint32_t f[4] = {pair_f16(lo, 0x4140), pair_f16(lo, 0x4342), pair_f16(hi, 0x4140), pair_f16(hi, 0x4342)};
+#pragma unroll
+                                    for (int n = 0; n < NT; n++) mma_f16(acc[n][2 * w + u], f, pb[h][n][0], pb[h][n][1]);
                                 }
                         }
-                        bool move = false;
-#pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            mx[c] = fmaxf(fmaxf(e[0][c], e[0][c + 2]), fmaxf(e[1][c], e[1][c + 2]));
-                            mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
-                            mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 8));
-                            mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 16));
-                            move |= mx[c] > m[n][c] + 8.f;
-                        }
-                        // the reference moves only when a score passes it by 2^8 (weights stay below 2^8)
-                        if (__any_sync(0xffffffffu, move)) {
-                            float alpha[2];
-#pragma unroll
-                            for (int c = 0; c < 2; c++) {
-                                const float mn = fmaxf(m[n][c], mx[c]);
-                                alpha[c] = m[n][c] == -INFINITY ? 0.f : ex2(m[n][c] - mn);
-                                m[n][c] = mn;
-                                l[n][c] *= alpha[c];
-                            }
-#pragma unroll
-                            for (int j = 0; j < 8; j++)
-#pragma unroll
-                                for (int x = 0; x < 4; x++) acc[n][j][x] *= alpha[x & 1];
-                        }
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-#pragma unroll
-                            for (int c = 0; c < 2; c++) {
-                                const float ref = m[n][c] == -INFINITY ? 0.f : m[n][c];
-                                e[h][c] = ex2(e[h][c] - ref);
-                                e[h][c + 2] = ex2(e[h][c + 2] - ref);
-                                l[n][c] = fmaf(e[h][c] + e[h][c + 2], iv[h], l[n][c]);
-                            }
-                            pb[h][n][0] = movmatrix_trans(pack2<__half>(e[h][0], e[h][1]));
-                            pb[h][n][1] = movmatrix_trans(pack2<__half>(e[h][2], e[h][3]));
-                        }
-                    }
-                    // O^T += V^T P^T: dimension 16 g + 2 j is the tile's row g, 16 g + 2 j + 1 its row g + 8. The V
-                    // fragments are signed integers (1024 + b + 128 - 1152): sums over thousands of keys would lose
-                    // what an offset left in them.
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint8_t* vp = kp + KS_HALF + h * PG_BLOCK * PG_DIM;
-                        const uint4 ra = *(const uint4*)(vp + v_off0), rb = *(const uint4*)(vp + v_off1);
-                        const uint4 rc = *(const uint4*)(vp + v_off0 + 8 * PG_DIM), rd = *(const uint4*)(vp + v_off1 + 8 * PG_DIM);
-                        const uint32_t va[4] = {ra.x, ra.y, ra.z, ra.w}, vb[4] = {rb.x, rb.y, rb.z, rb.w};
-                        const uint32_t vc[4] = {rc.x, rc.y, rc.z, rc.w}, vd[4] = {rd.x, rd.y, rd.z, rd.w};
-#pragma unroll
-                        for (int w = 0; w < 4; w++)
-#pragma unroll
-                            for (int u = 0; u < 2; u++) {
-                                const uint32_t sel = u ? 0x7362 : 0x5140;
-                                const uint32_t lo = __byte_perm(va[w], vb[w], sel) ^ 0x80808080u;
-                                const uint32_t hi = __byte_perm(vc[w], vd[w], sel) ^ 0x80808080u;
-                                const uint32_t f[4] = {pair_f16(lo, 0x4140), pair_f16(lo, 0x4342), pair_f16(hi, 0x4140), pair_f16(hi, 0x4342)};
-#pragma unroll
-                                for (int n = 0; n < NT; n++) mma_f16(acc[n][2 * w + u], f, pb[h][n][0], pb[h][n][1]);
-                            }
                     }
                 }
                 __syncwarp();
-                if (at * KS_KEYS < cur.hi)
-                    issue(cur, at++, issued++);
-                else if (nat * KS_KEYS < nxt.hi)
-                    issue(nxt, nat++, issued++);
+                out.next();
+                if (at * KEYS < cur.hi)
+                    issue(cur, at++, in);
+                else if (nat * KEYS < nxt.hi)
+                    issue(nxt, nat++, in);
+                else
+                    flight--;
             }
             // the chunk's result: lane (g, i) holds dimensions 16 g .. + 15 of rows 2 i and 2 i + 1
 #pragma unroll
@@ -433,17 +464,17 @@ __global__ void __launch_bounds__(KS_WARPS * 32, NT == 1 ? 3 : 2) k_kv8_small(At
                     }
                 }
         }
-        // what the next item still lacks of its first two stages (all of them after an item without keys)
+        // what the next item still lacks of its first stages (all of them after an item without keys)
         cur = nxt;
         at = nat;
-        while (issued - used < KS_STAGES && at * KS_KEYS < cur.hi) issue(cur, at++, issued++);
+        for (; flight < STAGES && at * KEYS < cur.hi; flight++) issue(cur, at++, in);
     }
 }
 
 // Joins the chunks of small requests: one CTA per (row, request, KV head), its warps over the chunks with a
-// running reference each, four chunks' loads in flight.
-constexpr int KJ_WARPS = 4;
-template <class T>
+// running reference each, four chunks' loads in flight. Latency-bound: 16 warps where a request can have more
+// than 128 chunks, else 4 (fewer idle warps per row).
+template <class T, int KJ_WARPS>
 __global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
     __shared__ float4 so[KJ_WARPS][32];
     __shared__ float2 sl[KJ_WARPS];
@@ -521,8 +552,8 @@ Workspace workspace(const jv_paged_batch& b, int kv_heads) {
 }
 
 // The cache as a 4-dimensional tensor of bytes, [page][kv head][K rows, V rows][128]; a box is the K or
-// the V of 32 tokens of one head. The encoder is looked up once through the runtime, so the library needs no link to libcuda.
-CUtensorMap page_map(const jv_kv8_cache& c) {
+// the V of `keys` tokens of one head. The encoder is looked up once through the runtime, so the library needs no link to libcuda.
+CUtensorMap page_map(const jv_kv8_cache& c, int keys) {
     using Encode = decltype(&cuTensorMapEncodeTiled);
     static const Encode encode = [] {
         void* p = nullptr;
@@ -534,7 +565,7 @@ CUtensorMap page_map(const jv_kv8_cache& c) {
     CUtensorMap m;
     const cuuint64_t dims[4] = {PG_DIM, 2 * PG_TOKENS, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
     const cuuint64_t strides[3] = {PG_DIM, 2 * PG_PLANE, (cuuint64_t)c.page_bytes};
-    const cuuint32_t box[4] = {PG_DIM, KS_KEYS, 1, 1}, ones[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {PG_DIM, (cuuint32_t)keys, 1, 1}, ones[4] = {1, 1, 1, 1};
     const CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, c.data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) throw Error(JV_ERR_DEVICE, "cuTensorMapEncodeTiled failed with " + std::to_string((int)r));
@@ -554,9 +585,10 @@ void allow_smem(int bytes) {
 }
 
 template <class T, int NT>
-void launch_small(const AttnKArgs& a, const CUtensorMap& map, int ctas, cudaStream_t s) {
-    allow_smem<k_kv8_small<T, NT>>(KS_SMEM);
-    launch_pdl(k_kv8_small<T, NT>, dim3(ctas), dim3(KS_WARPS * 32), KS_SMEM, s, a, map);
+void launch_small(const AttnKArgs& a, int ctas, cudaStream_t s) {
+    const CUtensorMap map = page_map(a.c, Ks<NT>::keys);
+    allow_smem<k_kv8_small<T, NT>>(Ks<NT>::smem);
+    launch_pdl(k_kv8_small<T, NT>, dim3(ctas), dim3(KS_WARPS * 32), Ks<NT>::smem, s, a, map);
     note_launch();
 }
 
@@ -566,14 +598,17 @@ void launch(const AttnKArgs& a, cudaStream_t s) {
     JV_CUDA(cudaGetDevice(&dev));
     JV_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     const int64_t small = a.v.small_cap * a.c.kv_heads;
-    const CUtensorMap map = page_map(a.c);
-    const int ctas = (int)std::min<int64_t>((small + KS_WARPS - 1) / KS_WARPS, (a.rows <= 8 ? 3 : 2) * sms);
+    const int ctas = (int)std::min<int64_t>((small + KS_WARPS - 1) / KS_WARPS, (a.rows <= 8 ? Ks<1>::ctas : Ks<2>::ctas) * sms);
     if (a.rows <= 8)
-        launch_small<T, 1>(a, map, ctas, s);
+        launch_small<T, 1>(a, ctas, s);
     else
-        launch_small<T, 2>(a, map, ctas, s);
+        launch_small<T, 2>(a, ctas, s);
     if (a.b.max_keys > PG_CHUNK) {
-        launch_pdl(k_kv8_join<T>, dim3(small_rows(a.b), a.b.requests, a.c.kv_heads), dim3(KJ_WARPS * 32), 0, s, a);
+        const dim3 grid(small_rows(a.b), a.b.requests, a.c.kv_heads);
+        if (a.b.max_blocks > 128 * 256 / PG_TOKENS)
+            launch_pdl(k_kv8_join<T, 16>, grid, dim3(16 * 32), 0, s, a);
+        else
+            launch_pdl(k_kv8_join<T, 4>, grid, dim3(4 * 32), 0, s, a);
         note_launch();
     }
 }

@@ -194,6 +194,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
     }
 #pragma unroll
     for (int j = 0; j < PLAN_PER; j++) {
+        if (j >= per) break;
         const long long total = (long long)old[j] + n_new[j];
         if (old[j] < 0 || n_new[j] < 0 || n_new[j] > b.max_new || total > (long long)b.max_blocks * PG_TOKENS) {
             bad = true;  // the step fails; its counts are left out
@@ -271,7 +272,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
 #pragma unroll
     for (int j = 0; j < PLAN_PER; j++) {
         const int r = r0 + j;
-        if (j >= per || r >= R) continue;
+        if (j >= per) break;
+        if (r >= R) continue;
         const Place q = {old[j], ok ? n_new[j] : 0, ok ? pre[0] : 0, ok ? pre[1] : 0, ok ? pre[2] : 0, ok ? pre[3] : 0, ok ? pre[4] : 0,
                          ok ? pre[5] : 0};
         b.lengths[r] = q.old + q.n_new;
