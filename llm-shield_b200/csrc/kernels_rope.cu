@@ -38,34 +38,13 @@ __device__ __forceinline__ void st1(__half* p, float v) { *p = __float2half_rn(v
 __device__ __forceinline__ void st1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // Four consecutive elements; one vector access when `vec` (the caller checked the alignment).
-__device__ __forceinline__ void ld4(const float* p, bool vec, float (&x)[4]) {
-    if (vec) {
-        const float4 v = *(const float4*)p;
-        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = p[e];
-    }
+__device__ __forceinline__ void get4(uint2 v, const __half*, float (&x)[4]) {
+    const float2 a = __half22float2(*(const __half2*)&v.x), b = __half22float2(*(const __half2*)&v.y);
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
 }
-__device__ __forceinline__ void ld4(const __half* p, bool vec, float (&x)[4]) {
-    if (vec) {
-        const uint2 v = *(const uint2*)p;
-        const float2 a = __half22float2(*(const __half2*)&v.x), b = __half22float2(*(const __half2*)&v.y);
-        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = __half2float(p[e]);
-    }
-}
-__device__ __forceinline__ void ld4(const __nv_bfloat16* p, bool vec, float (&x)[4]) {
-    if (vec) {
-        const uint2 v = *(const uint2*)p;
-        x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
-        x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = __bfloat162float(p[e]);
-    }
+__device__ __forceinline__ void get4(uint2 v, const __nv_bfloat16*, float (&x)[4]) {
+    x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
 }
 __device__ __forceinline__ void st4(float* p, bool vec, const float (&x)[4]) {
     if (vec) {
@@ -94,6 +73,29 @@ __device__ __forceinline__ void st4(__nv_bfloat16* p, bool vec, const float (&x)
     }
 }
 
+// Four elements as they are in memory, so that many rows can be in flight before the first is converted.
+template <class T>
+struct Quad {
+    uint2 raw;
+    __device__ __forceinline__ void load(const T* p, bool vec) {
+        if (vec) {
+            raw = *(const uint2*)p;
+        } else {
+            const uint16_t* h = (const uint16_t*)p;
+            raw = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+        }
+    }
+    __device__ __forceinline__ void get(float (&x)[4]) const { get4(raw, (const T*)nullptr, x); }
+};
+template <>
+struct Quad<float> {
+    float4 raw;
+    __device__ __forceinline__ void load(const float* p, bool vec) {
+        raw = vec ? *(const float4*)p : make_float4(p[0], p[1], p[2], p[3]);
+    }
+    __device__ __forceinline__ void get(float (&x)[4]) const { x[0] = raw.x, x[1] = raw.y, x[2] = raw.z, x[3] = raw.w; }
+};
+
 // ------------------------------------------------------------ rope
 
 struct RopeKArgs {
@@ -103,14 +105,16 @@ struct RopeKArgs {
     int tokens, dim, n_heads;  // n_heads: of both operands
 };
 
-constexpr int RP_TOKENS = 16;  // tokens per CTA
+constexpr int RP_TOKENS = 8;  // tokens per CTA
 
-// One CTA: up to 16 tokens, the heads [blockIdx.y * per_cta, + per_cta) of both operands. A thread
+// One CTA: up to 8 tokens, the heads [blockIdx.y * per_cta, + per_cta) of both operands. A thread
 // takes one pair of one head at a time (any layout, stride and alignment).
 template <class T>
 __global__ void __launch_bounds__(RP_THREADS) k_rope(RopeKArgs a, int per_cta) {
     __shared__ float2 cs[RP_TOKENS][128];
     __shared__ float temp[RP_TOKENS];
+    pdl_wait();
+    pdl_launch_dependents();
     const int t0 = blockIdx.x * RP_TOKENS, nt = min(RP_TOKENS, a.tokens - t0);
     const int half = a.spec.rotary_dim >> 1;
     for (int i = threadIdx.x; i < nt * half; i += RP_THREADS) {
@@ -144,72 +148,138 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope(RopeKArgs a, int per_cta) {
 }
 
 // The same with 16-byte accesses (V elements), for rows and pair halves that start on 16 bytes. A
-// "piece" is V consecutive elements: of adjacent pairs, or both halves of V half-split pairs, or V elements
-// behind rotary_dim. L lanes (a power of two) take a head's pieces.
+// "piece" is V consecutive elements of adjacent pairs, or both halves of V half-split pairs, or, in a second
+// sweep, V elements behind rotary_dim; a power of two of lanes takes a head's pieces, so that every lane of a
+// warp has the same kind. Bound by HBM: four (token, head) rows per thread in flight, the first four before
+// the angles are worked out. 8191 tokens x 40 heads of 128 in bf16, half of them turned: see the case table.
 template <class T>
 union Vec {
     uint4 raw;
     T e[16 / sizeof(T)];
 };
+__device__ __forceinline__ void rotate_vec(Vec<float>& u, Vec<float>& v, const float2* cs, bool half_split, float k) {
+#pragma unroll
+    for (int e = 0; e < 4; e += half_split ? 1 : 2) {
+        float& pa = u.e[e];
+        float& pb = half_split ? v.e[e] : u.e[e + 1];
+        const float2 c = cs[half_split ? e : e >> 1];
+        const float x = pa, y = pb;
+        pa = fmaf(-y, c.y, x * c.x) * k;
+        pb = fmaf(x, c.y, y * c.x) * k;
+    }
+}
+// 16-bit elements, two at a time: (u0, u1) and (v0, v1) of half-split pairs, (u0, u1) a pair itself otherwise.
+template <class T>
+__device__ __forceinline__ void rotate_vec(Vec<T>& u, Vec<T>& v, const float2* cs, bool half_split, float k) {
+    uint32_t* pu = (uint32_t*)&u.raw;
+    uint32_t* pv = (uint32_t*)&v.raw;
+#pragma unroll
+    for (int w = 0; w < 4; w += 2) {
+        float x[4], y[4];
+        get4(make_uint2(pu[w], pu[w + 1]), (const T*)nullptr, x);
+        if (half_split) {
+            get4(make_uint2(pv[w], pv[w + 1]), (const T*)nullptr, y);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float2 c = cs[2 * w + e];
+                const float r = fmaf(-y[e], c.y, x[e] * c.x);
+                y[e] = fmaf(x[e], c.y, y[e] * c.x);
+                x[e] = r;
+            }
+            if (k != 1.f)
+                for (int e = 0; e < 4; e++) y[e] *= k;
+            st4((T*)(pv + w), true, y);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const float2 c = cs[w + e / 2];
+                const float r = fmaf(-x[e + 1], c.y, x[e] * c.x);
+                x[e + 1] = fmaf(x[e], c.y, x[e + 1] * c.x);
+                x[e] = r;
+            }
+        }
+        if (k != 1.f)
+            for (int e = 0; e < 4; e++) x[e] *= k;
+        st4((T*)(pu + w), true, x);
+    }
+}
+template <class T>
+__device__ __forceinline__ void scale_vec(Vec<T>& u, float k) {
+#pragma unroll
+    for (int e = 0; e < (int)(16 / sizeof(T)); e++) st1(u.e + e, ld1(u.e + e) * k);
+}
+
 template <class T, int LAYOUT>
-__global__ void __launch_bounds__(RP_THREADS) k_rope_vec(RopeKArgs a, int per_cta, int lane_bits) {
-    constexpr int V = 16 / sizeof(T);
+__global__ void __launch_bounds__(RP_THREADS) k_rope_vec(RopeKArgs a, int per_cta, int turn_bits, int rest_bits) {
+    constexpr int V = 16 / sizeof(T), U = 4;
+    constexpr bool SPLIT = LAYOUT == JV_ROPE_HALF;
     __shared__ __align__(16) float2 cs[RP_TOKENS][128];
     __shared__ float temp[RP_TOKENS];
+    pdl_wait();
+    pdl_launch_dependents();
     const int t0 = blockIdx.x * RP_TOKENS, nt = min(RP_TOKENS, a.tokens - t0);
     const int half = a.spec.rotary_dim >> 1;
     const int h0 = blockIdx.y * per_cta, nh = min(per_cta, a.n_heads - h0);
-    const int piece = threadIdx.x & ((1 << lane_bits) - 1), step = RP_THREADS >> lane_bits;
-    const int turned = LAYOUT == JV_ROPE_HALF ? half / V : 2 * half / V;  // pieces that are rotated
-    const int pieces = turned + (a.dim - 2 * half) / V;
-    const bool rotate = piece < turned;
-    const int e0 = rotate || LAYOUT == JV_ROPE_ADJACENT ? piece * V : 2 * half + (piece - turned) * V;
+    Vec<T> u[U], v[U];
+    T* out[U];
+    int tt[U];  // a row's token, 256 added where it takes the query temperature; 255 without a row
+    int t, h, dt, dh, e0;
+    bool in_range;
+    auto begin = [&](int bits, int pieces, int first) {
+        const int piece = threadIdx.x & ((1 << bits) - 1), row = threadIdx.x >> bits, step = RP_THREADS >> bits;
+        e0 = first + piece * V;
+        in_range = piece < pieces;
+        t = row / nh, h = row % nh, dt = step / nh, dh = step % nh;
+    };
+    auto load = [&](bool turn) {
+#pragma unroll
+        for (int n = 0; n < U; n++) {
+            tt[n] = 255;
+            if (t < nt && in_range) {
+                const bool second = h0 + h >= a.x[0].heads;
+                const jv_heads& x = a.x[second ? 1 : 0];
+                const int hh = second ? h0 + h - a.x[0].heads : h0 + h;
+                const T* in = (const T*)x.in + (int64_t)(t0 + t) * x.in_token + (int64_t)hh * x.in_head + e0;
+                out[n] = (T*)x.out + (int64_t)(t0 + t) * x.out_token + (int64_t)hh * x.out_head + e0;
+                tt[n] = t | (x.temperature ? 256 : 0);
+                u[n].raw = *(const uint4*)in;
+                if (SPLIT && turn) v[n].raw = *(const uint4*)(in + half);
+            }
+            t += dt;
+            h += dh;
+            if (h >= nh) h -= nh, t++;
+        }
+    };
+    begin(turn_bits, SPLIT ? half / V : 2 * half / V, 0);
+    load(true);
     for (int i = threadIdx.x; i < nt * half; i += RP_THREADS) {
-        const int t = i / half, f = i % half;
-        cs[t][f] = rope_angle(a.spec.turns[f], a.positions[t0 + t], a.spec.mscale);
+        const int ti = i / half, f = i % half;
+        cs[ti][f] = rope_angle(a.spec.turns[f], a.positions[t0 + ti], a.spec.mscale);
     }
     if (threadIdx.x < nt)
         temp[threadIdx.x] = rope_temperature(a.positions[t0 + threadIdx.x], a.spec.temperature_ctx, a.spec.temperature_scale);
     __syncthreads();
-    if (piece >= pieces) return;
-    int i = threadIdx.x >> lane_bits, t = i / nh, h = i % nh;
-    const int dt = step / nh, dh = step % nh;
-#pragma unroll 4
-    for (; t < nt;) {
-        const bool second = h0 + h >= a.x[0].heads;
-        const jv_heads& x = a.x[second ? 1 : 0];
-        const int hh = second ? h0 + h - a.x[0].heads : h0 + h;
-        const T* in = (const T*)x.in + (int64_t)(t0 + t) * x.in_token + (int64_t)hh * x.in_head + e0;
-        T* out = (T*)x.out + (int64_t)(t0 + t) * x.out_token + (int64_t)hh * x.out_head + e0;
-        const float k = x.temperature ? temp[t] : 1.f;
-        Vec<T> u, v;
-        u.raw = *(const uint4*)in;
-        if (LAYOUT == JV_ROPE_HALF && rotate) {
-            v.raw = *(const uint4*)(in + half);
+    while (tt[0] != 255) {
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float2 c = cs[t][e0 + e];
-                const float p = ld1(u.e + e), q = ld1(v.e + e);
-                st1(u.e + e, __fsub_rn(__fmul_rn(p, c.x), __fmul_rn(q, c.y)) * k);
-                st1(v.e + e, __fadd_rn(__fmul_rn(p, c.y), __fmul_rn(q, c.x)) * k);
-            }
-            *(uint4*)(out + half) = v.raw;
-        } else if (LAYOUT == JV_ROPE_ADJACENT && rotate) {
-#pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                const float2 c = cs[t][(e0 + e) >> 1];
-                const float p = ld1(u.e + e), q = ld1(u.e + e + 1);
-                st1(u.e + e, __fsub_rn(__fmul_rn(p, c.x), __fmul_rn(q, c.y)) * k);
-                st1(u.e + e + 1, __fadd_rn(__fmul_rn(p, c.y), __fmul_rn(q, c.x)) * k);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; e++) st1(u.e + e, ld1(u.e + e) * k);
+        for (int n = 0; n < U; n++) {
+            if (tt[n] == 255) break;
+            rotate_vec(u[n], v[n], cs[tt[n] & 255] + (SPLIT ? e0 : e0 >> 1), SPLIT, tt[n] & 256 ? temp[tt[n] & 255] : 1.f);
+            *(uint4*)out[n] = u[n].raw;
+            if (SPLIT) *(uint4*)(out[n] + half) = v[n].raw;
         }
-        *(uint4*)out = u.raw;
-        t += dt;
-        h += dh;
-        if (h >= nh) h -= nh, t++;
+        load(true);
+    }
+    if (a.dim == 2 * half) return;
+    begin(rest_bits, (a.dim - 2 * half) / V, 2 * half);
+    load(false);
+    while (tt[0] != 255) {
+#pragma unroll
+        for (int n = 0; n < U; n++) {
+            if (tt[n] == 255) break;
+            if (tt[n] & 256) scale_vec(u[n], temp[tt[n] & 255]);
+            *(uint4*)out[n] = u[n].raw;
+        }
+        load(false);
     }
 }
 
@@ -221,7 +291,7 @@ struct AppendArgs {
     PlanView v;
     jv_heads k, vv, q;
     jv_rope_spec spec;
-    bool rope, kvec, vvec, qvec;  // vec: four elements at once
+    bool rope;
     int q_heads;                  // 0 without q
 };
 
@@ -253,28 +323,75 @@ __device__ __forceinline__ void rope4(float (&x)[4], const float2* cs, int layou
     }
 }
 
+// The largest magnitude of four values, as the integer that its bits are: not finite from 0x7f800000 on.
+__device__ __forceinline__ uint32_t top4(const float (&x)[4]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
+    return m;
+}
+__device__ __forceinline__ void finite4(const float (&x)[4], float& amax) {
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (fabsf(x[e]) < INFINITY) amax = fmaxf(amax, fabsf(x[e]));
+}
+// A block's scale and what its values are multiplied by, from each lane's largest magnitude and the scale the
+// block had. Where a value is not finite (false), `again` takes the largest of the others.
+template <class F>
+__device__ __forceinline__ bool block_scale(uint32_t top, float had, float& scale, float& inv, F&& again) {
+    top = __reduce_max_sync(0xffffffffu, top);
+    const bool finite = top < 0x7f800000u;
+    float amax = __uint_as_float(top);
+    if (!finite) {
+        amax = 0.f;
+        again(amax);
+        amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+    }
+    if (amax < 7.888609e-31f) amax = 0.f;  // 2^-100: 127 / amax stays finite
+    scale = __fdiv_rn(amax, 127.f);
+    inv = amax > 0.f ? __fdiv_rn(127.f, amax) : 0.f;
+    if (had > scale) {
+        scale = had;
+        inv = __fdiv_rn(1.f, had);
+    }
+    return finite;
+}
+// x inv rounded to a whole number by adding 1.5 2^23 (|x inv| <= 127, or it is clamped): the low byte of the sum
+// is the int8. Four of them in a word.
+__device__ __forceinline__ uint32_t quantise4(const float (&x)[4], float inv, bool finite) {
+    uint32_t q[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        float y = __fmul_rn(x[e], inv);
+        if (!finite) y = isnan(x[e]) || inv == 0.f ? 0.f : fminf(fmaxf(y, -127.f), 127.f);
+        q[e] = __float_as_uint(__fadd_rn(y, 12582912.f));
+    }
+    return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+}
+
 // One CTA: a 16-token block that the step writes to, a slice of its heads; one warp a head at a time
 // (a lane holds 4 dimensions of the 16 tokens, so a block's largest magnitude is one register
 // reduction and one shuffle tree).
-template <class T, class TQ>
-__global__ void __launch_bounds__(RP_THREADS) k_kv8_append(AppendArgs a) {
+template <class T, class TQ, bool VEC, bool ROPE>
+__global__ void __launch_bounds__(RP_THREADS, 2) k_kv8_append(AppendArgs a) {
     __shared__ float2 cs[PG_BLOCK][64];
     __shared__ float temp[PG_BLOCK];
+    pdl_wait();
+    pdl_launch_dependents();
     if ((int)blockIdx.x >= a.v.head[2]) return;
-    const int2 unit = a.v.units[blockIdx.x];
-    RequestRows rr;
-    if (!request_rows(a.b, unit.x, rr)) return;
-    const int p0 = unit.y * PG_BLOCK, old = rr.len - rr.n_new;
-    const int lo = max(0, old - p0), hi = min(PG_BLOCK, rr.len - p0);  // rows [lo, hi) are new, [0, lo) kept
-    if (p0 < 0 || lo >= hi || hi <= 0) return;
+    const int4 unit = a.v.units[blockIdx.x];
+    // rows [lo, hi) of the block are new, token tok0 + row each; [0, lo) are kept
+    const int p0 = unit.y * PG_BLOCK, tok0 = unit.z, lo = unit.w & 255, hi = unit.w >> 8;
+    if ((unsigned)unit.x >= (unsigned)a.b.requests || (unsigned)unit.y >= (unsigned)a.b.max_blocks * (PG_TOKENS / PG_BLOCK) || lo >= hi ||
+        hi > PG_BLOCK || tok0 + lo < 0 || tok0 > a.b.max_tokens - hi)
+        return;
     const int page = a.b.block_table[(int64_t)unit.x * a.b.max_blocks + p0 / PG_TOKENS];
     if ((unsigned)page >= (unsigned)a.c.pages) {
         if (threadIdx.x == 0) paged_report(a.b.status, JV_ERR_RANGE, PS_APPEND_PAGE);
         return;
     }
-    const int tok0 = rr.start + p0 - old;  // token of row 0 (rows from lo on exist)
     const int half = a.spec.rotary_dim >> 1;
-    if (a.rope) {
+    if (ROPE) {
         for (int i = threadIdx.x; i < PG_BLOCK * half; i += RP_THREADS) {
             const int t = i / half, f = i % half;
             if (t >= lo && t < hi) cs[t][f] = rope_angle(a.spec.turns[f], p0 + t, a.spec.mscale);
@@ -286,86 +403,105 @@ __global__ void __launch_bounds__(RP_THREADS) k_kv8_append(AppendArgs a) {
     const int lane = threadIdx.x & 31, g = a.c.kv_heads;
     const int n_work = 2 * g + a.q_heads;
     for (int w = blockIdx.y * (RP_THREADS / 32) + (threadIdx.x >> 5); w < n_work; w += gridDim.y * (RP_THREADS / 32)) {
-        if (w >= 2 * g) {  // a query head: rotate and hand on
+        if (ROPE && w >= 2 * g) {  // a query head: rotate and hand on
             const int h = w - 2 * g;
             bool bad = false;
-#pragma unroll 4
-            for (int t = 0; t < PG_BLOCK; t++) {
-                if (t < lo || t >= hi) continue;
-                float x[4];
-                ld4((const T*)a.q.in + (int64_t)(tok0 + t) * a.q.in_token + (int64_t)h * a.q.in_head + 4 * lane, a.qvec, x);
-                rope4(x, cs[t], a.spec.layout, half, lane);
-                const float k = a.q.temperature ? temp[t] : 1.f;
+            const T* in = (const T*)a.q.in + (int64_t)tok0 * a.q.in_token + (int64_t)h * a.q.in_head + 4 * lane;
+            TQ* out = (TQ*)a.q.out + (int64_t)tok0 * a.q.out_token + (int64_t)h * a.q.out_head + 4 * lane;
+            for (int t0 = lo; t0 < hi; t0 += 8) {
+                Quad<T> r[8];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    x[e] *= k;
-                    if (std::is_same<TQ, __half>::value) bad |= f16_out_of_range(x[e]);
+                for (int t = 0; t < 8; t++)
+                    if (t0 + t < hi) r[t].load(in + (t0 + t) * a.q.in_token, VEC);
+#pragma unroll
+                for (int t = 0; t < 8; t++) {
+                    if (t0 + t >= hi) break;
+                    float x[4];
+                    r[t].get(x);
+                    rope4(x, cs[t0 + t], a.spec.layout, half, lane);
+                    const float k = a.q.temperature ? temp[t0 + t] : 1.f;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        x[e] *= k;
+                        if (std::is_same<TQ, __half>::value) bad |= f16_out_of_range(x[e]);
+                    }
+                    st4(out + (t0 + t) * a.q.out_token, VEC, x);
                 }
-                st4((TQ*)a.q.out + (int64_t)(tok0 + t) * a.q.out_token + (int64_t)h * a.q.out_head + 4 * lane, a.qvec, x);
             }
             if (__any_sync(0xffffffffu, bad) && lane == 0) paged_report(a.b.status, JV_ERR_NUMERIC, PS_ROPE_VALUE);
             continue;
         }
         const int h = w >> 1, kv = w & 1;
         const jv_heads& src = kv ? a.vv : a.k;
-        float x[PG_BLOCK][4];
-        float amax = 0.f;
-        bool bad = false;
-#pragma unroll
-        for (int t = 0; t < PG_BLOCK; t++) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[t][e] = 0.f;
-            if (t >= lo && t < hi)
-                ld4((const T*)src.in + (int64_t)(tok0 + t) * src.in_token + (int64_t)h * src.in_head + 4 * lane,
-                    kv ? a.vvec : a.kvec, x[t]);
-        }
-#pragma unroll
-        for (int t = 0; t < PG_BLOCK; t++) {
-            if (a.rope && kv == 0 && t >= lo && t < hi) rope4(x[t], cs[t], a.spec.layout, half, lane);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float m = fabsf(x[t][e]);
-                if (m < INFINITY) {
-                    amax = fmaxf(amax, m);
-                } else {
-                    bad = true;
-                    if (isnan(x[t][e])) x[t][e] = 0.f;
-                }
-            }
-        }
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (__any_sync(0xffffffffu, bad) && lane == 0) paged_report(a.b.status, JV_ERR_NUMERIC, PS_APPEND_VALUE);
-        if (amax < 7.888609e-31f) amax = 0.f;  // 2^-100: 127 / amax stays finite
+        const bool turn = ROPE && kv == 0;
+        const T* in = (const T*)src.in + (int64_t)tok0 * src.in_token + (int64_t)h * src.in_head + 4 * lane;
         float* sp = a.c.scales + (int64_t)page * a.c.scale_stride + (h * 2 + kv) * 4 + (p0 % PG_TOKENS) / PG_BLOCK;
-        const float had = lo > 0 ? *sp : 0.f;
-        float scale = __fdiv_rn(amax, 127.f), inv = amax > 0.f ? __fdiv_rn(127.f, amax) : 0.f;
-        if (had > scale) {
-            scale = had;
-            inv = __fdiv_rn(1.f, had);
-        }
         char* dst = (char*)a.c.data + (int64_t)page * a.c.page_bytes + (int64_t)(h * 2 + kv) * PG_PLANE +
                     (p0 % PG_TOKENS) * PG_DIM + 4 * lane;
-        // values kept from earlier steps, at the grown scale (an 8-bit value again, off by half a step at most)
-        if (lo > 0 && had != scale) {
-            const float ratio = scale > 0.f ? __fdiv_rn(had, scale) : 0.f;
-#pragma unroll 1
-            for (int t = 0; t < lo; t++) {
-                char4 o = *(char4*)(dst + t * PG_DIM);
-                o.x = (signed char)rintf(o.x * ratio);
-                o.y = (signed char)rintf(o.y * ratio);
-                o.z = (signed char)rintf(o.z * ratio);
-                o.w = (signed char)rintf(o.w * ratio);
-                *(char4*)(dst + t * PG_DIM) = o;
+        float scale;
+        if (lo == 0 && hi == PG_BLOCK) {
+            // a whole block: its rows in registers, no entries to keep, no row to leave out
+            float x[PG_BLOCK][4];
+            {
+                Quad<T> raw[PG_BLOCK];
+#pragma unroll
+                for (int t = 0; t < PG_BLOCK; t++) raw[t].load(in + t * src.in_token, VEC);
+#pragma unroll
+                for (int t = 0; t < PG_BLOCK; t++) raw[t].get(x[t]);
             }
-        }
+            if (turn) {
 #pragma unroll
-        for (int t = 0; t < PG_BLOCK; t++) {
-            if (t < lo || t >= hi) continue;
-            int q[4];
+                for (int t = 0; t < PG_BLOCK; t++) rope4(x[t], cs[t], a.spec.layout, half, lane);
+            }
+            uint32_t top = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) q[e] = (int)fminf(fmaxf(rintf(__fmul_rn(x[t][e], inv)), -127.f), 127.f);
-            *(char4*)(dst + t * PG_DIM) = make_char4((signed char)q[0], (signed char)q[1], (signed char)q[2], (signed char)q[3]);
+            for (int t = 0; t < PG_BLOCK; t++) top = max(top, top4(x[t]));
+            float inv;
+            const bool finite = block_scale(top, 0.f, scale, inv, [&](float& amax) {
+#pragma unroll
+                for (int t = 0; t < PG_BLOCK; t++) finite4(x[t], amax);
+            });
+            if (!finite && lane == 0) paged_report(a.b.status, JV_ERR_NUMERIC, PS_APPEND_VALUE);
+#pragma unroll
+            for (int t = 0; t < PG_BLOCK; t++) *(uint32_t*)(dst + t * PG_DIM) = quantise4(x[t], inv, finite);
+        } else {
+            // part of a block: four rows at a time, read twice
+            auto rows = [&](auto&& use) {
+                for (int t0 = lo; t0 < hi; t0 += 4) {
+                    Quad<T> raw[4];
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+                        if (t0 + t < hi) raw[t].load(in + (t0 + t) * src.in_token, VEC);
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        if (t0 + t >= hi) break;
+                        float x[4];
+                        raw[t].get(x);
+                        if (turn) rope4(x, cs[t0 + t], a.spec.layout, half, lane);
+                        use(t0 + t, x);
+                    }
+                }
+            };
+            const float had = lo > 0 ? *sp : 0.f;
+            uint32_t top = 0;
+            rows([&](int, const float (&x)[4]) { top = max(top, top4(x)); });
+            float inv;
+            const bool finite = block_scale(top, had, scale, inv, [&](float& amax) { rows([&](int, const float (&x)[4]) { finite4(x, amax); }); });
+            if (!finite && lane == 0) paged_report(a.b.status, JV_ERR_NUMERIC, PS_APPEND_VALUE);
+            // values kept from earlier steps, at the grown scale (an 8-bit value again, off by half a step at most)
+            if (lo > 0 && had != scale) {
+                const float ratio = scale > 0.f ? __fdiv_rn(had, scale) : 0.f;
+#pragma unroll 4
+                for (int t = 0; t < lo; t++) {
+                    char4 o = *(char4*)(dst + t * PG_DIM);
+                    o.x = (signed char)rintf(o.x * ratio);
+                    o.y = (signed char)rintf(o.y * ratio);
+                    o.z = (signed char)rintf(o.z * ratio);
+                    o.w = (signed char)rintf(o.w * ratio);
+                    *(char4*)(dst + t * PG_DIM) = o;
+                }
+            }
+            rows([&](int t, const float (&x)[4]) { *(uint32_t*)(dst + t * PG_DIM) = quantise4(x, inv, finite); });
         }
         __syncwarp();
         if (lane == 0) *sp = scale;
@@ -406,27 +542,35 @@ void launch_rope(const RopeKArgs& a, int n, cudaStream_t s) {
               x.out_token % V == 0 && x.out_head % V == 0;
     }
     if (vec) {
-        const int pieces = (half_split ? a.dim - a.spec.rotary_dim / 2 : a.dim) / V;
-        int bits = 0;
-        while ((1 << bits) < pieces) bits++;
+        auto bits = [](int pieces) {
+            int b = 0;
+            while ((1 << b) < pieces) b++;
+            return b;
+        };
+        const int turn = bits(a.spec.rotary_dim / (half_split ? 2 * V : V)), rest = bits((a.dim - a.spec.rotary_dim) / V);
         if (half_split)
-            k_rope_vec<T, JV_ROPE_HALF><<<grid, RP_THREADS, 0, s>>>(a, per, bits);
+            launch_pdl(k_rope_vec<T, JV_ROPE_HALF>, grid, dim3(RP_THREADS), 0, s, a, per, turn, rest);
         else
-            k_rope_vec<T, JV_ROPE_ADJACENT><<<grid, RP_THREADS, 0, s>>>(a, per, bits);
+            launch_pdl(k_rope_vec<T, JV_ROPE_ADJACENT>, grid, dim3(RP_THREADS), 0, s, a, per, turn, rest);
     } else {
-        k_rope<T><<<grid, RP_THREADS, 0, s>>>(a, per);
+        launch_pdl(k_rope<T>, grid, dim3(RP_THREADS), 0, s, a, per);
     }
-    JV_CUDA(cudaGetLastError());
     note_launch();
 }
 
 template <class T, class TQ>
-void launch_append(const AppendArgs& a, cudaStream_t s) {
+void launch_append(const AppendArgs& a, bool vec, cudaStream_t s) {
+    // A head per warp, unless the angles that every CTA works out would then cost more than its heads: with
+    // rope, as many CTAs as fill the SMs.
     const int warps = RP_THREADS / 32, work = 2 * a.c.kv_heads + a.q_heads;
     const int most = (work + warps - 1) / warps;
-    const int split = (int)std::max<int64_t>(1, std::min<int64_t>(most, 592 / std::max<int64_t>(1, a.v.unit_cap)));
-    k_kv8_append<T, TQ><<<dim3((unsigned)a.v.unit_cap, split), RP_THREADS, 0, s>>>(a);
-    JV_CUDA(cudaGetLastError());
+    const int split = !a.rope ? most : (int)std::max<int64_t>(1, std::min<int64_t>(most, 592 / std::max<int64_t>(1, a.v.unit_cap)));
+    const dim3 grid((unsigned)a.v.unit_cap, split);
+    auto go = [&](auto kernel) { launch_pdl(kernel, grid, dim3(RP_THREADS), 0, s, a); };
+    if (a.rope)
+        vec ? go(k_kv8_append<T, TQ, true, true>) : go(k_kv8_append<T, TQ, false, true>);
+    else
+        vec ? go(k_kv8_append<T, __half, true, false>) : go(k_kv8_append<T, __half, false, false>);
     note_launch();
 }
 
@@ -536,8 +680,8 @@ int jv_kv8_append(const jv_kv8_cache* cache, const jv_paged_batch* batch, int32_
         a.v = plan_view(*batch);
         a.k = *k;
         a.vv = *v;
-        a.kvec = vec4(k->in, k->in_token, k->in_head, elem);
-        a.vvec = vec4(v->in, v->in_token, v->in_head, elem);
+        // four elements at once, where every operand's rows allow it
+        bool vec = vec4(k->in, k->in_token, k->in_head, elem) && vec4(v->in, v->in_token, v->in_head, elem);
         a.rope = rope != nullptr;
         if (rope) {
             check_spec(rope);
@@ -559,18 +703,18 @@ int jv_kv8_append(const jv_kv8_cache* cache, const jv_paged_batch* batch, int32_
                 throw Error(JV_ERR_ARG, "q in place must have the same type and strides in and out");
             a.q = *q;
             a.q_heads = q->heads;
-            a.qvec = vec4(q->in, q->in_token, q->in_head, elem) && vec4(q->out, q->out_token, q->out_head, oelem);
+            vec = vec && vec4(q->in, q->in_token, q->in_head, elem) && vec4(q->out, q->out_token, q->out_head, oelem);
         }
         OnDeviceOf dev(cache->data);
         cudaStream_t s = (cudaStream_t)stream;
         auto go = [&](auto t) {
             using T = decltype(t);
             if (!q || out_type == T_F16)
-                launch_append<T, __half>(a, s);
+                launch_append<T, __half>(a, vec, s);
             else if (out_type == T_F32)
-                launch_append<T, float>(a, s);
+                launch_append<T, float>(a, vec, s);
             else
-                launch_append<T, __nv_bfloat16>(a, s);
+                launch_append<T, __nv_bfloat16>(a, vec, s);
         };
         if (type == T_F32)
             go(float{});

@@ -103,7 +103,7 @@ PlanView plan_view(const jv_paged_batch& b) {
     v.prefix = (int32_t*)take(4 * R * 4);
     v.small_items = (int4*)take(v.small_cap * 32);
     v.large_items = (int4*)take(v.large_cap * 16);
-    v.units = (int2*)take(v.unit_cap * 8);
+    v.units = (int4*)take(v.unit_cap * 16);
     v.bytes = at;
     return v;
 }
@@ -159,7 +159,11 @@ __device__ __forceinline__ void plan_request(const PlanArgs& a, int r, const Pla
         b.slots[q.start + i] = (int64_t)page * PG_TOKENS + pos % PG_TOKENS;
     }
     const int units = units_of(q.old, q.n_new);
-    for (int i = t; i < units; i += n) a.v.units[q.unit + i] = make_int2(r, q.old / PG_BLOCK + i);
+    for (int i = t; i < units; i += n) {
+        const int block = q.old / PG_BLOCK + i, p0 = block * PG_BLOCK;
+        const int lo = max(0, q.old - p0), hi = min(PG_BLOCK, q.old + q.n_new - p0);
+        a.v.units[q.unit + i] = make_int4(r, block, q.start + p0 - q.old, lo | hi << 8);
+    }
     const int small = small_of(q.old, q.n_new, b.group), chunks = pg_chunks(q.old + q.n_new);
     for (int i = t; i < small; i += n) {
         a.v.small_items[2 * (q.small + i)] = make_int4(r, i % chunks, chunks, i / chunks);
@@ -179,6 +183,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
     __shared__ int ws[32][6];
     __shared__ long long wl[32][2];
     __shared__ Place places[PLAN_FILL_REQUESTS];
+    pdl_wait();
+    pdl_launch_dependents();
     const jv_paged_batch& b = a.b;
     const int R = b.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
     const int per = (R + blockDim.x - 1) / blockDim.x, r0 = tid * per;  // per <= PLAN_PER
@@ -314,6 +320,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(PlanArgs a, bool fill) {
 // The rest of a larger step: a CTA per request and slice of its tokens.
 __global__ void __launch_bounds__(PLAN_FILL_THREADS) k_plan_fill(PlanArgs a) {
     pdl_wait();
+    pdl_launch_dependents();
     const jv_paged_batch& b = a.b;
     const int r = blockIdx.x, R = b.requests;
     const int len = b.lengths[r], start = b.starts[r], n_new = b.starts[r + 1] - start;
@@ -339,6 +346,8 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <class T>
 __global__ void __launch_bounds__(256) k_kv8_read(jv_kv8_cache c, const int64_t* __restrict__ slots, int n, T* __restrict__ k_out,
                                                   T* __restrict__ v_out, int64_t row_stride, bool vec, int32_t* status) {
+    pdl_wait();
+    pdl_launch_dependents();
     const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
     const int part = threadIdx.x & 7;
     const int per = 2 * c.kv_heads;
@@ -381,8 +390,7 @@ void launch_read(const jv_kv8_cache& c, const int64_t* slots, int n, void* k, vo
                  cudaStream_t s) {
     const bool vec = aligned(k, 16) && aligned(v, 16) && stride * sizeof(T) % 16 == 0;
     const int64_t threads = (int64_t)n * 2 * c.kv_heads * 8;
-    k_kv8_read<T><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(c, slots, n, (T*)k, (T*)v, stride, vec, status);
-    JV_CUDA(cudaGetLastError());
+    launch_pdl(k_kv8_read<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, c, slots, n, (T*)k, (T*)v, stride, vec, status);
     note_launch();
 }
 
@@ -413,8 +421,7 @@ int jv_paged_plan(const jv_paged_batch* batch, const int32_t* cached, const int3
         // through them in less than a second launch costs (16 requests of one token: 3.9 us in one launch).
         const bool fill = batch->requests <= PLAN_FILL_REQUESTS && batch->max_new <= 256 && batch->max_tokens <= 4096;
         const int threads = batch->requests <= 8 ? 256 : PLAN_THREADS;
-        k_plan<<<1, threads, 0, (cudaStream_t)stream>>>(a, fill);
-        JV_CUDA(cudaGetLastError());
+        launch_pdl(k_plan, dim3(1), dim3(threads), 0, (cudaStream_t)stream, a, fill);
         note_launch();
         if (!fill) {
             const int slices = std::min(32, (batch->max_new + 1023) / 1024);

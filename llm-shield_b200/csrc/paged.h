@@ -51,7 +51,7 @@ struct PlanView {
     int32_t* prefix;    // [4][requests]: pages taken, units, large items and those with splits before request r
     int4* small_items;  // two each: {request, chunk, chunks, row tile}, {start, new, length, 0}; row tile by row tile
     int4* large_items;  // {request, pair of tiles, split, splits + 256 x place of its partials}; a pair's splits next to each other
-    int2* units;        // {request, block}: the 16-token blocks the step writes to
+    int4* units;        // the 16-token blocks the step writes to: {request, block, token of its row 0, first new row + 256 x end}
     int64_t small_cap, large_cap, split_cap, unit_cap, bytes;  // split_cap: most large items with more than one split
 };
 PlanView plan_view(const jv_paged_batch& b);

@@ -12,6 +12,7 @@ from ._lib import JvHeads, JvKv8Cache, JvPagedBatch, JvRopeSpec, check, lib
 PAGE_TOKENS, SCALE_TOKENS, HEAD_DIM = 64, 16, 128
 DTYPES = {"f32": 0, "f16": 1, "bf16": 30}
 LAYOUTS = {"interleaved": 0, "half": 1}
+_OPERANDS = [JvHeads * n for n in range(3)]
 SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
 
 
@@ -59,8 +60,8 @@ def heads(ptr: int, n_heads: int, token_stride: int, head_stride: int, out: int 
 
 def rope(spec: JvRopeSpec, dtype: str, positions: int, tokens: int, head_dim: int, *operands: JvHeads, stream: int = 0) -> None:
     """Rotates one or two operands (queries and keys) at positions[tokens] (jv_rope)."""
-    arr = (JvHeads * len(operands))(*operands)
-    check(lib.jv_rope(C.byref(spec), DTYPES[dtype], positions, tokens, head_dim, arr, len(operands), stream))
+    n = len(operands)
+    check(lib.jv_rope(C.byref(spec), DTYPES[dtype], positions, tokens, head_dim, _OPERANDS[n](*operands) if n <= 2 else None, n, stream))
 
 
 def cache(data: int, scales: int, pages: int, kv_heads: int, page_bytes: Optional[int] = None,
