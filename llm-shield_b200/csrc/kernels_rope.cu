@@ -439,8 +439,9 @@ __global__ void __launch_bounds__(RP_THREADS, 2) k_kv8_append(AppendArgs a) {
         char* dst = (char*)a.c.data + (int64_t)page * a.c.page_bytes + (int64_t)(h * 2 + kv) * PG_PLANE +
                     (p0 % PG_TOKENS) * PG_DIM + 4 * lane;
         float scale;
-        if (lo == 0 && hi == PG_BLOCK) {
-            // a whole block: its rows in registers, no entries to keep, no row to leave out
+        if (lo == 0 && hi == PG_BLOCK && !(ROPE && sizeof(T) == 4)) {
+            // a whole block: its rows in registers, no entries to keep, no row to leave out (fp32 rows with their
+            // angles would not fit: those go four at a time)
             float x[PG_BLOCK][4];
             {
                 Quad<T> raw[PG_BLOCK];

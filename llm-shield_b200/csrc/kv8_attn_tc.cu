@@ -5,16 +5,18 @@
 // One CTA = one KV head x a pair of query tiles A and B of 128 rows (128 / group tokens x the group's heads),
 // which share every block of 128 keys; per tile and block
 //   S = Q K^T   tcgen05.mma kind::f16, M = N = K = 128, S in TMEM (fp32)
-//   w = 2^(e - M) as fp16 pairs, over S in TMEM (a row per thread, M moves only past 2^8)
-//   O += W V    W as the TMEM operand, V from shared memory (MN-major)
-// TMEM: O_A, O_B, S_A / W_A, S_B / W_B, 128 columns each. S(b + 1) of a tile follows its W V(b) in the tensor
-// pipe, so S(b) complete means O holds the blocks before b; while one tile's rows are in the softmax the
-// other's products run.
+//   w = 2^(e - M) as fp16 to shared memory (a row per thread, M moves only past 2^8)
+//   O += W V    (V MN-major)
+// TMEM: O_A, O_B, S_A, S_B, 128 columns each. A softmax hands its S columns back as soon as it has them in
+// registers, so the next block's S runs under its exponentials, and each tile has its own W: the softmaxes
+// never wait for the tensor pipe but at the start. (W over S in TMEM, which saves the shared memory, measured
+// 5,900 cycles a block: S, softmax and W V one after the other, and both tiles in step.) What bounds it is the
+// exponential unit, 2,048 cycles a block of the two tiles, and the issue slots around it.
 // Warps 0-3 and 4-7: the softmax and output of tiles A and B. Warps 8-11: convert the cache's int8 to fp16
-// operands (K as b + 128 in subnormals, one byte permute; V signed), two stages of K and two of V, the next
-// block's bytes already in registers. Warps 12 and 13: issue tile A's and B's products. Registers are moved
-// from the last two warpgroups to the softmax (128 at launch: 184 + 184 + 104 + 40 = 4 x 128). Every wait is
-// bounded; on expiry the role records its site and stops.
+// operands (K as b + 128 in subnormals, one byte permute; V signed), two stages of K and one of V, in the
+// order K(b + 1), V(b), with the next blocks' bytes already in registers. Warps 12 and 13: issue tile A's and
+// B's products. Registers are moved from the last two warpgroups to the softmax (128 at launch: 184 + 184 +
+// 104 + 40 = 4 x 128). Every wait is bounded; on expiry the role records its site and stops.
 #include <atomic>
 
 #include <cuda_bf16.h>
@@ -29,7 +31,7 @@ constexpr int KT_THREADS = 512;
 constexpr int KT_KEYS = 128;
 constexpr int KT_TILE = 128 * 128 * 2;  // one fp16 operand tile
 constexpr int KT_SLOTS = 4;             // blocks whose scales are kept
-constexpr int KT_SMEM = 6 * KT_TILE + KT_SLOTS * 128 + 256 + 1024;
+constexpr int KT_SMEM = 7 * KT_TILE + KT_SLOTS * 128 + 256 + 1024;
 
 enum KtRole : int { KR_CONVERT_K = 0, KR_CONVERT_V = 1, KR_ISSUE = 2, KR_SOFTMAX = 3 };
 
@@ -38,12 +40,6 @@ __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.al
 template <int N>
 __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
 
-// A from TMEM.
-__device__ __forceinline__ void umma_ta(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-                 "r"(a), "l"(bd), "r"(idesc), "r"(acc)
-                 : "memory");
-}
 __device__ __forceinline__ bool elect_one() {
     uint32_t ok;
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
@@ -97,11 +93,12 @@ template <class T>
 __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
     extern __shared__ uint8_t kt_raw[];
     uint8_t* sm = kt_raw + ((1024u - (s_addr(kt_raw) & 1023u)) & 1023u);
+    // Q_A, Q_B, two K, V, W_A, W_B
     const uint32_t Qs = s_addr(sm), Ks = Qs + 2 * KT_TILE, Vs = Qs + 4 * KT_TILE;
-    float4* scales = (float4*)(sm + 6 * KT_TILE);  // [slot][8]: ks, log2 vs, 1 / vs of 16 keys
-    uint64_t* bars = (uint64_t*)(sm + 6 * KT_TILE + KT_SLOTS * 128);
-    const uint32_t k_full = s_addr(bars), v_full = k_full + 16, k_empty = k_full + 32, v_empty = k_full + 48;
-    const uint32_t q_full = k_full + 64, s_full = k_full + 80, p_full = k_full + 96, o_done = k_full + 112;
+    float4* scales = (float4*)(sm + 7 * KT_TILE);  // [slot][8]: ks, log2 vs, 1 / vs of 16 keys
+    uint64_t* bars = (uint64_t*)(sm + 7 * KT_TILE + KT_SLOTS * 128);
+    const uint32_t k_full = s_addr(bars), k_empty = k_full + 16, q_full = k_full + 32, s_full = k_full + 48;
+    const uint32_t s_free = k_full + 64, p_full = k_full + 80, o_done = k_full + 96, v_full = k_full + 112, v_empty = k_full + 120;
     uint32_t* tslot = (uint32_t*)(bars + 16);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -134,14 +131,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(k_full + 8 * i, 4);
-            mbar_init(v_full + 8 * i, 4);
             mbar_init(k_empty + 8 * i, 2);
-            mbar_init(v_empty + 8 * i, 2);
+            mbar_init(s_free + 8 * i, 4);
             mbar_init(q_full + 8 * i, 4);
             mbar_init(s_full + 8 * i, 1);
             mbar_init(p_full + 8 * i, 4);
             mbar_init(o_done + 8 * i, 1);
         }
+        mbar_init(v_full, 4);
+        mbar_init(v_empty, 2);
         fence_barrier_init();
     }
     if (warp == 12) tmem_alloc(s_addr(tslot), 512);
@@ -157,50 +155,66 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             // ------------------------------------------------ issue the products of one tile
             const int x = warp - 12;
             const uint32_t id_s = idesc_f16(KT_KEYS, PG_TILE), id_o = idesc_f16(PG_DIM, PG_TILE) | (1u << 16);
-            const uint32_t q = Qs + x * KT_TILE, o = tmem + (uint32_t)(x * 128), d = tmem + 256u + (uint32_t)(x * 128);
+            const uint32_t q = Qs + x * KT_TILE, w = Qs + (5 + x) * KT_TILE, o = tmem + (uint32_t)(x * 128),
+                           d = tmem + 256u + (uint32_t)(x * 128);
+            const int b0 = it.b0[x], b1 = it.b1[x];
+            auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_poll(bar, parity)) != 0; };
+            // The other tile's block n: released at once, but not before it is there (a release counts for the
+            // stage's current use).
+            auto skip = [&](int n) {
+                if (!all_wait(k_full + 8 * (n & 1), (uint32_t)((n >> 1) & 1)) || !all_wait(v_full, (uint32_t)(n & 1))) return false;
+                if (lane == 0) {
+                    mbar_arrive(k_empty + 8 * (n & 1));
+                    mbar_arrive(v_empty);
+                }
+                __syncwarp();
+                return true;
+            };
+            auto issue_s = [&](int b) {
+                const int n = b - it.lo;
+                if (!all_wait(k_full + 8 * (n & 1), (uint32_t)((n >> 1) & 1))) return false;
+                if (b > b0 && !all_wait(s_free + 8 * x, (uint32_t)((b - 1 - b0) & 1))) return false;
+                tc_fence_after();
+                const uint32_t k = Ks + (n & 1) * KT_TILE;
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < 8; kk++) {
+                        const uint32_t off = (uint32_t)((kk >> 2) * 16384 + (kk & 3) * 32);
+                        umma(d, sdesc(q + off), sdesc(k + off), id_s, kk > 0 ? 1u : 0u);
+                    }
+                    umma_commit(s_full + 8 * x);
+                    umma_commit(k_empty + 8 * (n & 1));
+                }
+                __syncwarp();
+                return true;
+            };
+            auto issue_o = [&](int b) {
+                const int n = b - it.lo;
+                if (!all_wait(p_full + 8 * x, (uint32_t)((b - b0) & 1)) || !all_wait(v_full, (uint32_t)(n & 1))) return false;
+                tc_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < 8; kk++) {
+                        const uint32_t off = (uint32_t)((kk >> 2) * 16384 + (kk & 3) * 32);
+                        umma(o, sdesc(w + off), sdesc_mn(Vs + kk * 2048), id_o, b > b0 || kk > 0 ? 1u : 0u);
+                    }
+                    umma_commit(o_done + 8 * x);
+                    umma_commit(v_empty);
+                }
+                __syncwarp();
+                return true;
+            };
             bool ok = true;
-            if (it.b0[x] < it.b1[x]) ok = warp_wait(q_full + 8 * x, 0);
-            for (int b = it.lo, n = 0; b < it.hi && ok; b++, n++) {
-                const uint32_t st = n & 1, ph = (n >> 1) & 1;
-                const bool mine = b >= it.b0[x] && b < it.b1[x];
-                const uint32_t k = Ks + st * KT_TILE, v = Vs + st * KT_TILE;
-                ok = __all_sync(0xffffffffu, mbar_poll(k_full + 8 * st, ph));
-                if (!ok) break;
-                if (mine) {
-                    tc_fence_after();
-                    if (elect_one()) {
-#pragma unroll
-                        for (int kk = 0; kk < 8; kk++) {
-                            const uint32_t off = (uint32_t)((kk >> 2) * 16384 + (kk & 3) * 32);
-                            umma(d, sdesc(q + off), sdesc(k + off), id_s, kk > 0 ? 1u : 0u);
-                        }
-                        umma_commit(s_full + 8 * x);
-                        umma_commit(k_empty + 8 * st);
-                    }
-                    __syncwarp();
-                    ok = __all_sync(0xffffffffu, mbar_poll(p_full + 8 * x, (uint32_t)((b - it.b0[x]) & 1)));
-                    ok = ok && __all_sync(0xffffffffu, mbar_poll(v_full + 8 * st, ph));
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-#pragma unroll
-                        for (int kk = 0; kk < 8; kk++)
-                            umma_ta(o, d + (uint32_t)(8 * kk), sdesc_mn(v + kk * 2048), id_o, b > it.b0[x] || kk > 0 ? 1u : 0u);
-                        umma_commit(v_empty + 8 * st);
-                        if (b + 1 == it.b1[x]) umma_commit(o_done + 8 * x);
-                    }
-                    __syncwarp();
-                } else {
-                    // the other tile's block: released at once, but not before it is there (a release counts for
-                    // the stage's current use)
-                    ok = __all_sync(0xffffffffu, mbar_poll(v_full + 8 * st, ph));
-                    if (ok && lane == 0) {
-                        mbar_arrive(k_empty + 8 * st);
-                        mbar_arrive(v_empty + 8 * st);
-                    }
-                    __syncwarp();
+            int n = 0;
+            if (b0 < b1) {
+                for (; n < b0 - it.lo && ok; n++) ok = skip(n);
+                ok = ok && warp_wait(q_full + 8 * x, 0) && issue_s(b0);
+                for (int b = b0; b < b1 && ok; b++, n++) {
+                    if (b + 1 < b1) ok = issue_s(b + 1);
+                    ok = ok && issue_o(b);
                 }
             }
+            for (; n < it.hi - it.lo && ok; n++) ok = skip(n);
             if (!ok && lane == 0) paged_report(err, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_TC + KR_ISSUE);
         }
     } else if (warp >= 8) {
@@ -231,13 +245,11 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
                                            (r0 + 16 * (k & 3)) * PG_DIM + 16 * j);
             }
         };
-        int p0 = page_of(it.lo, 0), p1 = page_of(it.lo, 1);
-        int n0 = page_of(it.lo + 1, 0), n1 = page_of(it.lo + 1, 1);
-        load(kr, p0, p1, 0);
-        load(vr, p0, p1, 1);
-        bool ok = true;
-        for (int b = it.lo, n = 0; b < it.hi; b++, n++) {
-            const uint32_t st = n & 1, ph = ((n >> 1) & 1) ^ 1;
+        // Block n's keys and scales; its bytes are in kr, its pages p0 and p1. Loads the next block's.
+        int p0 = page_of(it.lo, 0), p1 = page_of(it.lo, 1);        // of the block whose K is next
+        int n0 = page_of(it.lo + 1, 0), n1 = page_of(it.lo + 1, 1);  // and of the one after it
+        auto keys = [&](int n) {
+            const int b = it.lo + n;
             float4 sc = make_float4(0.f, 0.f, 1.f, 0.f);  // without a page nothing is visible
             if (t < 8) {
                 const int id = t < 4 ? p0 : p1;
@@ -248,31 +260,40 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
                     sc = make_float4(s[0], lg2_approx(vs), __frcp_rn(vs), 0.f);
                 }
             }
-            ok = warp_wait(k_empty + 8 * st, ph);
-            if (!ok) {
+            if (!warp_wait(k_empty + 8 * (n & 1), (uint32_t)((n >> 1) & 1) ^ 1u)) {
                 if (lane == 0) paged_report(err, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_TC + KR_CONVERT_K);
-                break;
+                return false;
             }
             if (t < 8) scales[(n & (KT_SLOTS - 1)) * 8 + t] = sc;
 #pragma unroll
-            for (int k = 0; k < 8; k++) convert16<false>(Ks + st * KT_TILE, r0 + 16 * k, j, kr[k]);
+            for (int k = 0; k < 8; k++) convert16<false>(Ks + (n & 1) * KT_TILE, r0 + 16 * k, j, kr[k]);
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(k_full + 8 * st);
-            load(kr, n0, n1, 0);
-            ok = warp_wait(v_empty + 8 * st, ph);
+            if (lane == 0) mbar_arrive(k_full + 8 * (n & 1));
+            p0 = n0, p1 = n1;
+            load(kr, p0, p1, 0);
+            n0 = page_of(b + 2, 0), n1 = page_of(b + 2, 1);
+            return true;
+        };
+        load(kr, p0, p1, 0);
+        load(vr, p0, p1, 1);
+        const int blocks = it.hi - it.lo;
+        bool ok = blocks == 0 || keys(0);
+        for (int n = 0; n < blocks && ok; n++) {
+            const int v0 = p0, v1 = p1;  // the pages of block n + 1
+            if (n + 1 < blocks) ok = keys(n + 1);
+            if (!ok) break;
+            ok = warp_wait(v_empty, (uint32_t)(n & 1) ^ 1u);
             if (!ok) {
                 if (lane == 0) paged_report(err, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_TC + KR_CONVERT_V);
                 break;
             }
 #pragma unroll
-            for (int k = 0; k < 8; k++) convert16<true>(Vs + st * KT_TILE, r0 + 16 * k, j, vr[k]);
+            for (int k = 0; k < 8; k++) convert16<true>(Vs, r0 + 16 * k, j, vr[k]);
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(v_full + 8 * st);
-            load(vr, n0, n1, 1);
-            p0 = n0, p1 = n1;
-            n0 = page_of(b + 2, 0), n1 = page_of(b + 2, 1);
+            if (lane == 0) mbar_arrive(v_full);
+            if (n + 1 < blocks) load(vr, v0, v1, 1);
         }
     } else {
         reg_inc<184>();
@@ -355,6 +376,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
                 tld_wait(v2);
                 tld_wait(v3);
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_free + 8 * x);  // S(b + 1) may overwrite S(b)
             const int k0 = b * KT_KEYS, vis_hi = hi_key - k0, vis_lo = lo_key - k0;
             const bool all = __all_sync(0xffffffffu, vis_hi >= KT_KEYS && vis_lo <= 0);
             float bm = -INFINITY;
@@ -402,9 +426,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             }
             l = fmaf(l, alpha, rs);
             m = mn;
-            tst32(s_col, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-            tst32(s_col + 32u, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-            // O *= alpha where a row's reference moved (S(b) complete: so is W V(b - 1))
+            // W is free, and O holds every block before b, once W V(b - 1) is done
+            if (b > it.b0[x] && !warp_wait(o_done + 8 * x, (uint32_t)((b - 1 - it.b0[x]) & 1))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < 16; c++)
+                *(uint4*)(sm + (5 + x) * KT_TILE + tile_off(r, c)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+            // O *= alpha where a row's reference moved
             if (b > it.b0[x] && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
                 for (int h = 0; h < 4; h++) {
@@ -417,12 +448,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
                 }
             }
             tst_wait();
+            fence_proxy_async();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + 8 * x);
         }
         const bool any = it.b0[x] < it.b1[x];
-        if (ok && any) ok = warp_wait(o_done + 8 * x, 0);
+        if (ok && any) ok = warp_wait(o_done + 8 * x, (uint32_t)((it.b1[x] - 1 - it.b0[x]) & 1));
         if (!ok) {
             if (lane == 0) paged_report(err, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_TC + KR_SOFTMAX);
         } else {
