@@ -59,8 +59,8 @@ struct KtItem {
     int lo, hi;           // blocks of the CTA
 };
 
-// 16 int8 of one row (dimensions 16 j ..) as 32 bytes of fp16 into a [128][128] operand tile. Lanes 0-3 of a
-// row's eight store their even chunk first, lanes 4-7 their odd one, so that eight lanes meet eight chunks.
+// 16 int8 of one row (dimensions 16 j ..) as 32 bytes of fp16 into a [128][128] operand tile. Eight lanes that
+// store together hold four j of two neighbouring rows: eight different chunks.
 template <bool SIGNED>
 __device__ __forceinline__ void convert16(uint32_t tile, int row, int j, uint4 raw) {
     const uint32_t w[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};
@@ -78,15 +78,32 @@ __device__ __forceinline__ void convert16(uint32_t tile, int row, int j, uint4 r
             }
         }
     }
-    const bool flip = j >= 4;
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const int c = 2 * j + (flip ? 1 - k : k);
-        const uint32_t at = tile + tile_off(row, c);
-        const uint32_t x0 = flip == (k == 0) ? h[4] : h[0], x1 = flip == (k == 0) ? h[5] : h[1], x2 = flip == (k == 0) ? h[6] : h[2],
-                       x3 = flip == (k == 0) ? h[7] : h[3];
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(x0), "r"(x1), "r"(x2), "r"(x3) : "memory");
-    }
+    for (int k = 0; k < 2; k++)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(tile + tile_off(row, 2 * j + k)), "r"(h[4 * k]), "r"(h[4 * k + 1]),
+                     "r"(h[4 * k + 2]), "r"(h[4 * k + 3])
+                     : "memory");
+}
+// Packed fp32 pairs (a register pair each).
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
 }
 
 template <class T>
@@ -158,7 +175,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             const uint32_t q = Qs + x * KT_TILE, w = Qs + (5 + x) * KT_TILE, o = tmem + (uint32_t)(x * 128),
                            d = tmem + 256u + (uint32_t)(x * 128);
             const int b0 = it.b0[x], b1 = it.b1[x];
-            auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_poll(bar, parity)) != 0; };
+            auto all_wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity); };
             // The other tile's block n: released at once, but not before it is there (a release counts for the
             // stage's current use).
             auto skip = [&](int n) {
@@ -220,7 +237,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
     } else if (warp >= 8) {
         reg_dec<104>();
         // ---------------------------------------------------- int8 -> fp16 operands
-        const int t = tid - 256, j = t & 7, r0 = t >> 3;  // 16 bytes j of rows r0 + 16 k
+        const int t = tid - 256, j0 = t & 3, r0 = t >> 2;  // 16 bytes j0 and j0 + 4 of rows r0 + 32 k
         const int32_t* table = a.b.block_table + (int64_t)item.x * a.b.max_blocks;
         const int pages = (int)(((int64_t)it.rr.len + PG_TOKENS - 1) / PG_TOKENS);
         // the two pages of a block; -1 where the request has none
@@ -238,11 +255,11 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
         auto load = [&](uint4 (&r)[8], int p0, int p1, int plane) {
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const int id = k < 4 ? p0 : p1;
+                const int id = k < 4 ? p0 : p1;  // piece k: row r0 + 32 (k / 2), bytes 16 (j0 + 4 (k & 1))
                 r[k] = make_uint4(0, 0, 0, 0);
                 if (id >= 0)
                     r[k] = *(const uint4*)((const char*)a.c.data + (int64_t)id * a.c.page_bytes + (int64_t)(2 * kvh + plane) * PG_PLANE +
-                                           (r0 + 16 * (k & 3)) * PG_DIM + 16 * j);
+                                           (r0 + 32 * ((k >> 1) & 1)) * PG_DIM + 16 * (j0 + 4 * (k & 1)));
             }
         };
         // Block n's keys and scales; its bytes are in kr, its pages p0 and p1. Loads the next block's.
@@ -266,7 +283,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             }
             if (t < 8) scales[(n & (KT_SLOTS - 1)) * 8 + t] = sc;
 #pragma unroll
-            for (int k = 0; k < 8; k++) convert16<false>(Ks + (n & 1) * KT_TILE, r0 + 16 * k, j, kr[k]);
+            for (int k = 0; k < 8; k++) convert16<false>(Ks + (n & 1) * KT_TILE, r0 + 32 * (k >> 1), j0 + 4 * (k & 1), kr[k]);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(k_full + 8 * (n & 1));
@@ -289,7 +306,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
                 break;
             }
 #pragma unroll
-            for (int k = 0; k < 8; k++) convert16<true>(Vs, r0 + 16 * k, j, vr[k]);
+            for (int k = 0; k < 8; k++) convert16<true>(Vs, r0 + 32 * (k >> 1), j0 + 4 * (k & 1), vr[k]);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(v_full);
@@ -414,14 +431,18 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             for (int h = 0; h < 8; h++) {
                 const float4 s = sc[h];
                 const float ka = all ? s.x * qs : 1.f, kb = (all ? fmaf(s.x, qb, s.y) : 0.f) - ref;
-                float g = 0.f;
+                const uint64_t ka2 = pack_f32x2(ka, ka), kb2 = pack_f32x2(kb, kb);
+                uint64_t g2 = 0;
 #pragma unroll
                 for (int e = 16 * h; e < 16 * h + 16; e += 2) {
-                    const float w0 = ex2(fmaf(__uint_as_float(v[e]), ka, kb)), w1 = ex2(fmaf(__uint_as_float(v[e + 1]), ka, kb));
-                    g += w0 + w1;
+                    const float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), ka2, kb2));
+                    const float w0 = ex2(y.x), w1 = ex2(y.y);
+                    g2 = add_f32x2(g2, pack_f32x2(w0, w1));
                     const __half2 hp = __floats2half2_rn(w0, w1);
                     v[e >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
                 }
+                const float2 gs = unpack_f32x2(g2);
+                const float g = gs.x + gs.y;
                 rs = fmaf(g, s.z, rs);
             }
             l = fmaf(l, alpha, rs);
