@@ -15,8 +15,8 @@
 // Warps 0-3 and 4-7: the softmax and output of tiles A and B. Warps 8-11: convert the cache's int8 to fp16
 // operands (K as b + 128 in subnormals, one byte permute; V signed), two stages of K and one of V, in the
 // order K(b + 1), V(b), with the next blocks' bytes already in registers. Warps 12 and 13: issue tile A's and
-// B's products. Registers are moved from the last two warpgroups to the softmax (128 at launch: 184 + 184 +
-// 104 + 40 = 4 x 128). Every wait is bounded; on expiry the role records its site and stops.
+// B's products. Registers are moved from the last two warpgroups to the softmax (128 at launch: 192 + 192 +
+// 96 + 32 = 4 x 128). Every wait is bounded; on expiry the role records its site and stops.
 #include <atomic>
 
 #include <cuda_bf16.h>
@@ -83,6 +83,11 @@ __device__ __forceinline__ void convert16(uint32_t tile, int row, int j, uint4 r
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(tile + tile_off(row, 2 * j + k)), "r"(h[4 * k]), "r"(h[4 * k + 1]),
                      "r"(h[4 * k + 2]), "r"(h[4 * k + 3])
                      : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 // Packed fp32 pairs (a register pair each).
 __device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
@@ -167,7 +172,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
     int* err = a.b.status;
 
     if (warp >= 12) {
-        reg_dec<40>();
+        reg_dec<32>();
         if (warp < 14) {
             // ------------------------------------------------ issue the products of one tile
             const int x = warp - 12;
@@ -235,7 +240,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             if (!ok && lane == 0) paged_report(err, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_TC + KR_ISSUE);
         }
     } else if (warp >= 8) {
-        reg_dec<104>();
+        reg_dec<96>();
         // ---------------------------------------------------- int8 -> fp16 operands
         const int t = tid - 256, j0 = t & 3, r0 = t >> 2;  // 16 bytes j0 and j0 + 4 of rows r0 + 32 k
         const int32_t* table = a.b.block_table + (int64_t)item.x * a.b.max_blocks;
@@ -313,18 +318,19 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             if (n + 1 < blocks) load(vr, v0, v1, 1);
         }
     } else {
-        reg_inc<184>();
+        reg_inc<192>();
         // ---------------------------------------------------- softmax and output, a query row per thread
         const int x = warp >> 2, r = tid & 127;
+        const int b0 = it.b0[x], b1 = it.b1[x], nt = it.nt[x], t0 = it.t0[x];
         const int tok = r / group, j = r - tok * group;
-        const bool live = tok < it.nt[x];
-        const int pos = it.rr.len - it.rr.n_new + it.t0[x] + tok;
+        const bool live = tok < nt;
+        const int pos = it.rr.len - it.rr.n_new + t0 + tok;
         // rows of no token see everything: they are not stored, and must not send their warp down the masked path
         const int hi_key = live ? pos + 1 : 1 << 30, lo_key = live && a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-        const int64_t token = it.rr.start + it.t0[x] + tok;
+        const int64_t token = it.rr.start + t0 + tok;
         const int head = kvh * group + j;
         float qs = 0.f, qb = 0.f;
-        if (it.b0[x] < it.b1[x]) {
+        if (b0 < b1) {
             // the row to shared memory as fp16 (bf16: times a power of two, as in kv8_attn.cu), and its sum
             uint32_t w[64];
 #pragma unroll
@@ -371,8 +377,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
         const uint32_t o_col = tmem + lanes + (uint32_t)(x * 128), s_col = tmem + lanes + 256u + (uint32_t)(x * 128);
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int b = it.b0[x]; b < it.b1[x]; b++) {
-            if (!warp_wait(s_full + 8 * x, (uint32_t)((b - it.b0[x]) & 1))) {
+        for (int b = b0; b < b1; b++) {
+            if (!warp_wait(s_full + 8 * x, (uint32_t)((b - b0) & 1))) {
                 ok = false;
                 break;
             }
@@ -416,9 +422,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
 #pragma unroll
                 for (int h = 0; h < 8; h++) {
                     const float4 s = sc[h];
-                    float g = __uint_as_float(v[16 * h]);
+                    // three inputs at a time, in two chains
+                    float g = max3(__uint_as_float(v[16 * h]), __uint_as_float(v[16 * h + 1]), __uint_as_float(v[16 * h + 2]));
+                    float g1 = max3(__uint_as_float(v[16 * h + 3]), __uint_as_float(v[16 * h + 4]), __uint_as_float(v[16 * h + 5]));
 #pragma unroll
-                    for (int e = 16 * h + 1; e < 16 * h + 16; e++) g = fmaxf(g, __uint_as_float(v[e]));
+                    for (int e = 16 * h + 6; e < 16 * h + 14; e += 4) {
+                        g = max3(g, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                        g1 = max3(g1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+                    }
+                    g = max3(fmaxf(g, g1), __uint_as_float(v[16 * h + 14]), __uint_as_float(v[16 * h + 15]));
                     bm = fmaxf(bm, fmaf(g, s.x * qs, fmaf(s.x, qb, s.y)));
                 }
             }
@@ -448,7 +460,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             l = fmaf(l, alpha, rs);
             m = mn;
             // W is free, and O holds every block before b, once W V(b - 1) is done
-            if (b > it.b0[x] && !warp_wait(o_done + 8 * x, (uint32_t)((b - 1 - it.b0[x]) & 1))) {
+            if (b > b0 && !warp_wait(o_done + 8 * x, (uint32_t)((b - 1 - b0) & 1))) {
                 ok = false;
                 break;
             }
@@ -457,7 +469,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             for (int c = 0; c < 16; c++)
                 *(uint4*)(sm + (5 + x) * KT_TILE + tile_off(r, c)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
             // O *= alpha where a row's reference moved
-            if (b > it.b0[x] && __any_sync(0xffffffffu, alpha != 1.f)) {
+            if (b > b0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
                 for (int h = 0; h < 4; h++) {
                     uint32_t o[32];
@@ -474,8 +486,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + 8 * x);
         }
-        const bool any = it.b0[x] < it.b1[x];
-        if (ok && any) ok = warp_wait(o_done + 8 * x, (uint32_t)((it.b1[x] - 1 - it.b0[x]) & 1));
+        const bool any = b0 < b1;
+        if (ok && any) ok = warp_wait(o_done + 8 * x, (uint32_t)((b1 - 1 - b0) & 1));
         if (!ok) {
             if (lane == 0) paged_report(err, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_TC + KR_SOFTMAX);
         } else {
