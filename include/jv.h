@@ -44,6 +44,7 @@ enum jv_status {
 typedef struct jv_model jv_model;       /* weights resident on one device            */
 typedef struct jv_ctx jv_ctx;           /* MinistralModel instance: KV cache + stream */
 typedef struct jv_snapshot jv_snapshot; /* refcounted KV pages of a prefix            */
+typedef struct jv_server jv_server;     /* many requests over one 8-bit KV cache      */
 
 /* ModelConfig (src/Jevstral/Model/ModelConfig.cs:11-56), plus the resolved RoPE magnitude
  * scale (Rope.MagnitudeScale, src/Jevstral/Model/Rope.cs:28) and the weight type. */
@@ -336,6 +337,30 @@ int64_t jv_kv8_attention_bytes(const jv_paged_batch* batch, int32_t kv_heads);
  * the batch. Rows of q start on 16 bytes. */
 int jv_kv8_attention(const jv_kv8_cache* cache, const jv_paged_batch* batch, int32_t type, const jv_heads* q, float scale,
                      int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- many requests of one model, stepped together (no counterpart in the reference) ------
+ * A jv_server holds an 8-bit KV cache (the paged-batch section above: half the bytes per position
+ * of a context's fp16 pages) for up to max_requests requests, and runs the new tokens of any of
+ * them in one pass: one product per weight matrix for all, plan, rotation and append, attention,
+ * and the head's rows at each request's last token. Like a jv_ctx it is single-threaded, and it
+ * shares the jv_model's weights. A request's results do not depend, bit for bit, on what else is in
+ * the pass. */
+
+/* max_context: most positions of a request; max_tokens: most new tokens of one pass; pages: pages of
+ * 64 positions shared by the requests (0 = max_context positions for every request). */
+int jv_server_create(jv_model* model, int32_t max_requests, int32_t max_context, int32_t max_tokens, int32_t pages,
+                     jv_server** out);
+void jv_server_destroy(jv_server* server);
+/* One pass: request r brings counts[r] tokens (0: it sits the pass out), back to back in `tokens` in
+ * request order. out[requests with tokens][n_rows] = logits of vocabulary `rows` at each one's last
+ * token, in request order. JV_ERR_OOM when the pages run out and JV_ERR_RANGE when a request would
+ * pass max_context leave every request as it was. */
+int jv_server_forward(jv_server* server, const int32_t* tokens, const int32_t* counts, const int32_t* rows,
+                      int32_t n_rows, float* out);
+/* Ends a request: its positions go to 0 and its pages back to the others. */
+int jv_server_release(jv_server* server, int32_t request);
+int32_t jv_server_length(const jv_server* server, int32_t request); /* positions held; -1 for a bad index */
+int64_t jv_server_bytes_per_position(const jv_server* server);
 
 /* ---- KV cache (src/Jevstral/Model/KvCache.cs) ----------------------------------------- */
 

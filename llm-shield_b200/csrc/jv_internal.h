@@ -359,6 +359,7 @@ void launch_add(float* h, const float* x, int64_t n, cudaStream_t s);
 void launch_head_rows(const QWeight& table, const float* normed, int n_out, const int32_t* rows, int n_rows,
                       float* out, int* err, cudaStream_t s);
 void launch_argmax(const float* x, int n, int32_t* out, cudaStream_t s);
+void launch_f16_to_kslab(const __half* x, int T, int K, int tpad, __half* xs, cudaStream_t s);
 void launch_kslab_to_f32(const __half* xs, int T, int K, int tpad, float* out, cudaStream_t s);
 // KV pages <-> the reference's flat fp32 snapshot layout (keys of every layer/head, then values).
 // Elements [base, base + count) of the flat snapshot (count = 0: to the end), to or from a

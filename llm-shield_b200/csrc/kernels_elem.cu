@@ -307,6 +307,23 @@ void launch_kslab_to_f32(const __half* xs, int T, int K, int tpad, float* out, c
     note_launch();
 }
 
+// fp16 [T][K] -> the K-slab operand, 16 bytes at a time.
+__global__ void k_f16_to_kslab(const __half* __restrict__ x, int T, int K, int tpad, __half* __restrict__ xs) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int per = K / 8;
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= (int64_t)T * per) return;
+    const int t = (int)(i / per), k = (int)(i % per) * 8;
+    *(uint4*)(xs + kslab_offset(t, k, tpad)) = *(const uint4*)(x + (int64_t)t * K + k);
+}
+
+void launch_f16_to_kslab(const __half* x, int T, int K, int tpad, __half* xs, cudaStream_t s) {
+    const int64_t n = (int64_t)T * (K / 8);
+    launch_pdl(k_f16_to_kslab, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, x, T, K, tpad, xs);
+    note_launch();
+}
+
 }  // namespace jv
 
 namespace jv {

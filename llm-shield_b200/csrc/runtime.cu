@@ -16,11 +16,13 @@
 #include <limits>
 #include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
 #include "gguf.h"
 #include "jv_internal.h"
+#include "paged.h"
 
 using namespace jv;
 
@@ -1405,6 +1407,157 @@ HostLayout layout_tree(int start, int trunk, const std::vector<int>& offsets, in
 
 }  // namespace
 
+// Many requests over one 8-bit cache (the jv_server section of jv.h). The pass runs on an inner context's stream
+// and buffers; pages are taken on the device by jv_paged_plan, whose rule (from the end of the free list, in
+// request order) the host repeats on its own copy, so that a release needs no read-back.
+struct jv_server {
+    jv_model* m = nullptr;
+    jv_ctx* x = nullptr;
+    int max_requests = 0, max_context = 0, max_tokens = 0, max_blocks = 0, pages = 0;
+    std::vector<int32_t> lengths, free_pages;
+    std::vector<std::vector<int32_t>> table;  // pages of each request
+    bool dirty = true;                        // the host's state is ahead of the device's
+    jv_rope_spec rope{};
+    jv_paged_batch batch{};
+    std::vector<jv_kv8_cache> layers;
+    int64_t page_bytes = 0, scale_stride = 0, ws_bytes = 0;
+    DevVec<uint8_t> data, work, ws;
+    DevVec<float> scales;
+    DevVec<int32_t> d_table, d_lengths, d_starts, d_request, d_positions, d_free, d_counts, d_status;  // counts: new, n_free
+    DevVec<int64_t> d_slots;
+    DevVec<__half> attn;
+};
+
+namespace {
+
+void rc_check(int rc) {
+    if (rc != JV_OK) throw Error(rc, g_last_error);
+}
+
+void server_upload(jv_server* v) {
+    std::vector<int32_t> t((size_t)v->max_requests * v->max_blocks, 0);
+    for (int r = 0; r < v->max_requests; r++) std::copy(v->table[r].begin(), v->table[r].end(), t.begin() + (size_t)r * v->max_blocks);
+    const int32_t n_free = (int32_t)v->free_pages.size();
+    cudaStream_t s = v->x->stream;
+    JV_CUDA(cudaMemcpyAsync(v->d_table.p, t.data(), t.size() * 4, cudaMemcpyHostToDevice, s));
+    JV_CUDA(cudaMemcpyAsync(v->d_lengths.p, v->lengths.data(), v->lengths.size() * 4, cudaMemcpyHostToDevice, s));
+    if (n_free > 0) JV_CUDA(cudaMemcpyAsync(v->d_free.p, v->free_pages.data(), (size_t)n_free * 4, cudaMemcpyHostToDevice, s));
+    JV_CUDA(cudaMemcpyAsync(v->d_counts.p + v->max_requests, &n_free, 4, cudaMemcpyHostToDevice, s));
+    JV_CUDA(cudaStreamSynchronize(s));  // the host vectors go
+    v->dirty = false;
+}
+
+void server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, const int32_t* rows, int n_rows, float* out) {
+    jv_model* m = v->m;
+    jv_ctx* x = v->x;
+    const jv_config& c = m->cfg;
+    set_device(m);
+    // checks, before anything changes
+    int64_t T = 0, need = 0;
+    std::vector<int32_t> outputs;
+    for (int r = 0; r < v->max_requests; r++) {
+        if (counts[r] < 0) throw Error(JV_ERR_ARG, "request " + std::to_string(r) + " has a negative token count");
+        const int64_t len = (int64_t)v->lengths[r] + counts[r];
+        if (len > v->max_context)
+            throw Error(JV_ERR_RANGE, "request " + std::to_string(r) + " would pass its " + std::to_string(v->max_context) + " positions");
+        need += (len + PG_TOKENS - 1) / PG_TOKENS - (int64_t)v->table[r].size();
+        T += counts[r];
+        if (counts[r] > 0) outputs.push_back((int32_t)(T - 1));
+    }
+    if (T == 0) throw Error(JV_ERR_ARG, "No tokens to forward.");
+    if (T > v->max_tokens) throw Error(JV_ERR_RANGE, "more than " + std::to_string(v->max_tokens) + " tokens in one pass");
+    if (need > (int64_t)v->free_pages.size())
+        throw Error(JV_ERR_OOM, "the server's cache has no pages left (" + std::to_string(v->pages) + " of 64 positions)");
+    for (int64_t i = 0; i < T; i++)
+        if ((unsigned)tokens[i] >= (unsigned)m->embd.rows)
+            throw Error(JV_ERR_RANGE, "Token id " + std::to_string(tokens[i]) + " is outside the " + std::to_string(m->embd.rows) +
+                                          "-entry embedding table.");
+    for (int i = 0; i < n_rows; i++)
+        if ((unsigned)rows[i] >= (unsigned)m->head.rows)
+            throw Error(JV_ERR_RANGE, "vocabulary row " + std::to_string(rows[i]) + " is out of range");
+    check_cancel(x);
+
+    const int n = (int)T, n_out = (int)outputs.size();
+    const int hidden = c.hidden, qdim = c.heads * c.head_dim, kvdim = c.kv_heads * c.head_dim, qkvn = qdim + 2 * kvdim, ff = c.ff;
+    const int tpad = gemm_tpad_for(n);
+    cudaStream_t s = x->stream;
+    // one upload: tokens, outputs, rows, counts
+    const size_t words = (size_t)n + n_out + n_rows + v->max_requests;
+    int32_t* hin = x->h_in.get(words);
+    int32_t* din = x->in_i32.get(words);
+    std::memcpy(hin, tokens, 4 * (size_t)n);
+    std::memcpy(hin + n, outputs.data(), 4 * (size_t)n_out);
+    std::memcpy(hin + n + n_out, rows, 4 * (size_t)n_rows);
+    std::memcpy(hin + n + n_out + n_rows, counts, 4 * (size_t)v->max_requests);
+    // every buffer before the first launch: growing one frees the old
+    float* h = x->h.get((size_t)n * hidden);
+    float* qkv = x->qkv32.get((size_t)n * qkvn);
+    __half* xs = x->xs.get((size_t)tpad * hidden);
+    __half* q16 = x->q16.get((size_t)n * qdim);
+    __half* attn = v->attn.get((size_t)n * qdim);
+    __half* ctx16 = x->ctx16.get((size_t)tpad * qdim);
+    __half* xf = x->xs_ff.get((size_t)tpad * ff);
+    if (v->dirty) server_upload(v);
+    v->dirty = true;  // until the pass has gone through
+    JV_CUDA(cudaMemcpyAsync(din, hin, 4 * words, cudaMemcpyHostToDevice, s));
+    rc_check(jv_paged_plan(&v->batch, v->d_lengths.p, din + n + n_out + n_rows, v->d_free.p, v->d_counts.p + v->max_requests,
+                           v->d_counts.p + v->max_requests, s));
+    launch_embed(m->embd, din, n, h, hidden, x->d_err, s);
+    const float* resid = nullptr;
+    for (int l = 0; l < c.layers; l++) {
+        check_cancel(x);
+        const LayerW& W = m->layers[l];
+        launch_rmsnorm_resid(h, resid, W.attn_norm, n, hidden, c.eps, xs, tpad, x->d_err, s);
+        gemm(x, W.qkv, xs, n, tpad, qkv, qkvn, EPI_STORE);
+        // q, k and v are slices of the projection's fp32 rows
+        const jv_heads hq = {qkv, q16, qkvn, 128, qdim, 128, c.heads, 1};
+        const jv_heads hk = {qkv + qdim, nullptr, qkvn, 128, 0, 0, c.kv_heads, 0};
+        const jv_heads hv = {qkv + qdim + kvdim, nullptr, qkvn, 128, 0, 0, c.kv_heads, 0};
+        rc_check(jv_kv8_append(&v->layers[l], &v->batch, T_F32, &hk, &hv, &v->rope, &hq, T_F16, s));
+        const jv_heads ha = {q16, attn, qdim, 128, qdim, 128, c.heads, 0};
+        rc_check(jv_kv8_attention(&v->layers[l], &v->batch, T_F16, &ha, 1.f / std::sqrt((float)c.head_dim), 0, v->ws.p, v->ws_bytes, s));
+        launch_f16_to_kslab(attn, n, qdim, tpad, ctx16, s);
+        resid = gemm_resid(x, W.o, ctx16, n, tpad, h, hidden);
+        launch_rmsnorm_resid(h, resid, W.ffn_norm, n, hidden, c.eps, xs, tpad, x->d_err, s);
+        gemm(x, W.gu, xs, n, tpad, nullptr, 2 * ff, EPI_SWIGLU, xf);
+        resid = gemm_resid(x, W.down, xf, n, tpad, h, hidden);
+    }
+    if (resid) launch_resid_add(h, resid, (int64_t)n * hidden, s);
+    float* hres = nullptr;
+    if (n_rows > 0) {
+        float* normed = x->x32.get((size_t)n_out * hidden);
+        launch_rmsnorm_rows(h, din + n, n_out, m->out_norm, hidden, c.eps, normed, nullptr, 0, x->d_err, s);
+        float* d_res = x->out32.get((size_t)n_out * n_rows);
+        launch_head_rows(m->head, normed, n_out, din + n + n_out, n_rows, d_res, x->d_err, s);
+        hres = x->h_out.get((size_t)n_out * n_rows);
+        JV_CUDA(cudaMemcpyAsync(hres, d_res, sizeof(float) * n_out * n_rows, cudaMemcpyDeviceToHost, s));
+    }
+    int32_t status[2] = {0, 0};
+    JV_CUDA(cudaMemcpyAsync(status, v->d_status.p, sizeof status, cudaMemcpyDeviceToHost, s));
+    sync_check(x);
+    if (status[0] != 0) {
+        JV_CUDA(cudaMemsetAsync(v->d_status.p, 0, sizeof status, s));
+        JV_CUDA(cudaStreamSynchronize(s));
+        throw Error(status[0], status[0] == JV_ERR_NUMERIC
+                                   ? "a rotated query, or a key or value for the 8-bit cache, is not in the fp16 range or not a number"
+                               : status[0] == JV_ERR_DEVICE_TIMEOUT ? "a device-side wait timed out (attention over the 8-bit cache)"
+                                                                    : "a paged-batch operator refused the pass (site " + std::to_string(status[1]) + ")");
+    }
+    // the pass went through: the device's lengths, tables and free list are the host's
+    for (int r = 0; r < v->max_requests; r++) {
+        v->lengths[r] += counts[r];
+        while ((int)v->table[r].size() * PG_TOKENS < v->lengths[r]) {
+            v->table[r].push_back(v->free_pages.back());
+            v->free_pages.pop_back();
+        }
+    }
+    v->dirty = false;
+    if (n_rows > 0) std::memcpy(out, hres, sizeof(float) * n_out * n_rows);
+    x->resolve_profile();
+}
+
+}  // namespace
+
 namespace jv {
 int api_error(int code, const std::string& msg) { return set_error(code, msg); }
 
@@ -1780,6 +1933,116 @@ int jv_decode_greedy(jv_ctx* x, int32_t first_token, int32_t steps, int32_t* out
         std::memcpy(out_tokens, hres, sizeof(int32_t) * steps);
         x->length = end;
     });
+}
+
+int jv_server_create(jv_model* m, int32_t max_requests, int32_t max_context, int32_t max_tokens, int32_t pages, jv_server** out) {
+    if (!m || !out) return set_error(JV_ERR_ARG, "NULL argument");
+    *out = nullptr;
+    jv_server* v = new (std::nothrow) jv_server();
+    if (!v) return set_error(JV_ERR_OOM, "host memory exhausted");
+    v->m = m;
+    int rc = guarded([&] {
+        const jv_config& c = m->cfg;
+        if (max_requests < 1 || max_requests > PG_MAX_REQUESTS) throw Error(JV_ERR_ARG, "max_requests must be 1 to 4096");
+        if (max_context < 1 || max_context > m->rope_positions)
+            throw Error(JV_ERR_ARG, "max_context must be 1 to the model's " + std::to_string(m->rope_positions) + " positions");
+        if (max_tokens < 1 || max_tokens > (1 << 20)) throw Error(JV_ERR_ARG, "max_tokens must be 1 to 2^20");
+        if (pages < 0) throw Error(JV_ERR_ARG, "pages is negative");
+        const int blocks = (max_context + PG_TOKENS - 1) / PG_TOKENS;
+        const int64_t all = (int64_t)blocks * max_requests;
+        if (pages == 0 && all > INT32_MAX) throw Error(JV_ERR_ARG, "max_requests x max_context is too large");
+        set_device(m);
+        v->max_requests = max_requests, v->max_context = max_context, v->max_blocks = blocks;
+        v->max_tokens = max_tokens, v->pages = pages > 0 ? pages : (int)all;
+        v->lengths.assign(max_requests, 0);
+        v->table.resize(max_requests);
+        for (int i = v->pages - 1; i >= 0; i--) v->free_pages.push_back(i);
+        // the model's own frequencies (fp32, YaRN mixed in when active), in turns
+        v->rope.layout = JV_ROPE_ADJACENT;
+        v->rope.rotary_dim = c.rope_dim;
+        v->rope.mscale = m->mscale;
+        v->rope.temperature_scale = c.temperature_scale;
+        v->rope.temperature_ctx = c.rope_orig_ctx;
+        for (int i = 0; i < c.rope_dim / 2; i++) v->rope.turns[i] = (double)m->freqs[i] / 6.283185307179586476925286766559;
+        v->page_bytes = (int64_t)c.layers * c.kv_heads * 2 * PG_PLANE;
+        v->scale_stride = (int64_t)c.layers * c.kv_heads * 8;
+        jv_ctx* x = nullptr;
+        rc_check(jv_ctx_create(m, 1, &x));
+        v->x = x;
+        ctx_release_pages(x);  // its own fp16 pages are not used
+        jv_paged_batch& b = v->batch;
+        b.requests = max_requests;
+        b.max_new = std::min(max_context, max_tokens);
+        b.max_tokens = max_tokens;
+        b.max_blocks = blocks;
+        b.max_keys = std::min<int64_t>((int64_t)v->pages * PG_TOKENS, all * PG_TOKENS);
+        b.group = c.heads / c.kv_heads;
+        b.pages = v->pages;
+        const int64_t wb = jv_paged_work_bytes(&b);
+        v->ws_bytes = jv_kv8_attention_bytes(&b, c.kv_heads);
+        if (wb < 0 || v->ws_bytes < 0) throw Error(JV_ERR_ARG, g_last_error);
+        b.block_table = v->d_table.get((size_t)all);
+        b.lengths = v->d_lengths.get(max_requests);
+        b.starts = v->d_starts.get(max_requests + 1);
+        b.request_of = v->d_request.get(max_tokens);
+        b.positions = v->d_positions.get(max_tokens);
+        b.slots = v->d_slots.get(max_tokens);
+        b.work = v->work.get((size_t)wb);
+        b.status = v->d_status.get(2);
+        v->d_free.get(v->pages);
+        v->d_counts.get(max_requests + 1);
+        v->ws.get((size_t)v->ws_bytes);
+        uint8_t* data = v->data.get((size_t)v->pages * v->page_bytes);
+        float* scales = v->scales.get((size_t)v->pages * v->scale_stride);
+        for (int l = 0; l < c.layers; l++)
+            v->layers.push_back({data + (int64_t)l * c.kv_heads * 2 * PG_PLANE, scales + (int64_t)l * c.kv_heads * 8, v->page_bytes,
+                                 v->scale_stride, v->pages, c.kv_heads});
+    });
+    if (rc != JV_OK) {
+        const std::string msg = g_last_error;
+        jv_server_destroy(v);
+        return set_error(rc, msg);
+    }
+    *out = v;
+    return JV_OK;
+}
+
+void jv_server_destroy(jv_server* v) {
+    if (!v) return;
+    cudaSetDevice(v->m->device);
+    if (v->x) cudaStreamSynchronize(v->x->stream);
+    for (auto* d : {&v->data, &v->work, &v->ws}) d->release();
+    for (auto* d : {&v->d_table, &v->d_lengths, &v->d_starts, &v->d_request, &v->d_positions, &v->d_free, &v->d_counts, &v->d_status})
+        d->release();
+    v->scales.release();
+    v->d_slots.release();
+    v->attn.release();
+    if (v->x) jv_ctx_destroy(v->x);
+    delete v;
+}
+
+int jv_server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, const int32_t* rows, int32_t n_rows, float* out) {
+    if (!v || !tokens || !counts || n_rows < 0 || (n_rows > 0 && (!rows || !out))) return set_error(JV_ERR_ARG, "NULL argument");
+    return guarded([&] { server_forward(v, tokens, counts, rows, n_rows, out); });
+}
+
+int jv_server_release(jv_server* v, int32_t request) {
+    if (!v) return set_error(JV_ERR_ARG, "NULL argument");
+    if (request < 0 || request >= v->max_requests) return set_error(JV_ERR_RANGE, "no such request");
+    return guarded([&] {
+        v->free_pages.insert(v->free_pages.end(), v->table[request].rbegin(), v->table[request].rend());
+        v->table[request].clear();
+        v->lengths[request] = 0;
+        v->dirty = true;
+    });
+}
+
+int32_t jv_server_length(const jv_server* v, int32_t request) {
+    return v && request >= 0 && request < v->max_requests ? v->lengths[request] : -1;
+}
+
+int64_t jv_server_bytes_per_position(const jv_server* v) {
+    return v ? (v->page_bytes + v->scale_stride * 4) / PG_TOKENS : 0;
 }
 
 int32_t jv_kv_length(jv_ctx* x) { return x ? x->length : 0; }

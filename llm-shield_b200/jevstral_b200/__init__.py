@@ -10,5 +10,5 @@ from ._lib import (ArgumentError, ArgumentOutOfRangeError, DeviceError, DeviceOu
 from .decider import (DecisionResult, TokenDecider, decision_probs, margins_from_verdicts,  # noqa: F401
                       softmax)
 from .layout import TokenLayout  # noqa: F401
-from .model import KvCache, MinistralModel, Model, ModelConfig, Snapshot, device_count, kernel_launches  # noqa: F401
+from .model import KvCache, MinistralModel, Model, ModelConfig, Server, Snapshot, device_count, kernel_launches  # noqa: F401
 from . import dp, paged  # noqa: F401,E402

@@ -99,6 +99,12 @@ SIGNATURES = [
     ("jv_kv8_attention_bytes", i64, [C.POINTER(JvPagedBatch), i32]),
     ("jv_kv8_attention", C.c_int, [C.POINTER(JvKv8Cache), C.POINTER(JvPagedBatch), i32, C.POINTER(JvHeads), C.c_float,
                                    i32, vp, i64, vp]),
+    ("jv_server_create", C.c_int, [vp, i32, i32, i32, i32, C.POINTER(vp)]),
+    ("jv_server_destroy", None, [vp]),
+    ("jv_server_forward", C.c_int, [vp, i32p, i32p, i32p, i32, f32p]),
+    ("jv_server_release", C.c_int, [vp, i32]),
+    ("jv_server_length", i32, [vp, i32]),
+    ("jv_server_bytes_per_position", i64, [vp]),
     ("jv_kv_length", i32, [vp]),
     ("jv_kv_capacity", i32, [vp]),
     ("jv_kv_reset", C.c_int, [vp]),

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
-from typing import Callable, List, Optional, Sequence, Tuple
+from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -373,3 +373,51 @@ class MinistralModel:
         out = np.empty(steps, dtype=np.int32)
         check(lib.jv_decode_greedy(self._h, int(first_token), int(steps), _p(out)))
         return out
+
+
+class Server:
+    """Many requests of one model over one 8-bit KV cache (jv_server): each pass runs the new tokens of
+    any of them together. Not thread-safe, like a MinistralModel."""
+
+    def __init__(self, model: Model, max_requests: int, max_context: int, max_tokens: int, pages: int = 0):
+        h = C.c_void_p()
+        check(lib.jv_server_create(model._h, int(max_requests), int(max_context), int(max_tokens), int(pages), C.byref(h)))
+        self._h = h
+        self.model = model
+        self.max_requests = max_requests
+
+    def close(self) -> None:
+        if self._h:
+            lib.jv_server_destroy(self._h)
+            self._h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    @property
+    def bytes_per_position(self) -> int:
+        return int(lib.jv_server_bytes_per_position(self._h))
+
+    def length(self, request: int) -> int:
+        return int(lib.jv_server_length(self._h, int(request)))
+
+    def forward(self, tokens: Dict[int, Sequence[int]], vocab_rows: Sequence[int]) -> Dict[int, np.ndarray]:
+        """{request: its new tokens} -> {request: logits of vocab_rows at its last token}."""
+        counts = np.zeros(self.max_requests, dtype=np.int32)
+        for r, t in tokens.items():
+            if not 0 <= r < self.max_requests:
+                raise _lib.ArgumentOutOfRangeError(_lib.JV_ERR_RANGE, f"no request {r}")
+            counts[r] = len(t)
+        flat = _i32([x for r in sorted(tokens) for x in tokens[r]])
+        active = [r for r in sorted(tokens) if len(tokens[r])]
+        r = _i32(vocab_rows)
+        out = np.empty((len(active), r.size), dtype=np.float32)
+        check(lib.jv_server_forward(self._h, _p(flat), _p(counts), _p(r), r.size, _p(out, C.c_float)))
+        return dict(zip(active, out))
+
+    def release(self, request: int) -> None:
+        """Ends a request; its pages go back to the others."""
+        check(lib.jv_server_release(self._h, int(request)))

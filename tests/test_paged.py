@@ -180,3 +180,15 @@ def test_sizes_grow_with_the_bounds():
     b = _batch()
     assert lib.jv_kv8_attention_bytes(C.byref(b), 2) > 0
     assert lib.jv_kv8_attention_bytes(C.byref(b), 0) == -1
+
+
+def test_server_entry_points_check_their_handles():
+    from jevstral_b200._lib import JV_ERR_ARG, lib
+
+    h = C.c_void_p()
+    assert lib.jv_server_create(None, 1, 1, 1, 0, C.byref(h)) == JV_ERR_ARG
+    one = (C.c_int32 * 1)(1)
+    assert lib.jv_server_forward(None, one, one, one, 0, None) == JV_ERR_ARG
+    assert lib.jv_server_release(None, 0) == JV_ERR_ARG
+    assert lib.jv_server_length(None, 0) == -1 and lib.jv_server_bytes_per_position(None) == 0
+    lib.jv_server_destroy(None)
