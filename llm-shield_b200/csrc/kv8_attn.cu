@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(KS_WARPS * 32, Ks<NT>::ctas) k_kv8_small(AttnK
                   t.row0 < t.n_new * group && x.y >= 0 && x.z >= 1;
         if (!t.valid) t.n_new = t.len = t.row0 = 0;
         t.n_rows = min(min(t.n_new * group - t.row0, a.rows), 8 * NT);
-        const int ck = pg_chunk_keys(t.len);
+        const int ck = pg_chunk_keys(t.len, t.n_new * group);
         const int64_t from = (int64_t)x.y * ck;
         t.lo = (int)min(from, (int64_t)t.len);
         t.hi = (int)min(from + ck, (int64_t)t.len);
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
     const int row = blockIdx.x, request = blockIdx.y, kvh = blockIdx.z;
     RequestRows rr;
     if (!request_rows(a.b, request, rr)) return;
-    const int n_rows = rr.n_new * a.b.group, chunks = pg_chunks(rr.len);
+    const int n_rows = rr.n_new * a.b.group, chunks = pg_chunks(rr.len, n_rows);
     if (n_rows > PG_SMALL_ROWS || row >= n_rows || chunks < 2) return;
     const int first = a.v.first[request], item0 = first + row / PG_ROW_TILE * chunks;
     if (first < 0 || item0 + chunks > a.v.small_cap) return;

@@ -138,7 +138,7 @@ __device__ __forceinline__ int pages_of(int old, int n_new) {
 }
 __device__ __forceinline__ bool is_small(int n_new, int group) { return (int64_t)n_new * group <= PG_SMALL_ROWS; }
 __device__ __forceinline__ int small_of(int old, int n_new, int group) {
-    return n_new > 0 && is_small(n_new, group) ? pg_chunks(old + n_new) * ((n_new * group + PG_ROW_TILE - 1) / PG_ROW_TILE) : 0;
+    return n_new > 0 && is_small(n_new, group) ? pg_chunks(old + n_new, n_new * group) * ((n_new * group + PG_ROW_TILE - 1) / PG_ROW_TILE) : 0;
 }
 __device__ __forceinline__ int large_of(int old, int n_new, int group) {
     return n_new > 0 && !is_small(n_new, group) ? pg_pairs(n_new, group) * pg_splits(old + n_new, pg_pairs(n_new, group)) : 0;
@@ -164,7 +164,7 @@ __device__ __forceinline__ void plan_request(const PlanArgs& a, int r, const Pla
         const int lo = max(0, q.old - p0), hi = min(PG_BLOCK, q.old + q.n_new - p0);
         a.v.units[q.unit + i] = make_int4(r, block, q.start + p0 - q.old, lo | hi << 8);
     }
-    const int small = small_of(q.old, q.n_new, b.group), chunks = pg_chunks(q.old + q.n_new);
+    const int small = small_of(q.old, q.n_new, b.group), chunks = pg_chunks(q.old + q.n_new, q.n_new * b.group);
     for (int i = t; i < small; i += n) {
         a.v.small_items[2 * (q.small + i)] = make_int4(r, i % chunks, chunks, i / chunks);
         a.v.small_items[2 * (q.small + i) + 1] = make_int4(q.start, q.n_new, q.old + q.n_new, 0);

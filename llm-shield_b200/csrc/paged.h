@@ -21,17 +21,17 @@ constexpr int PG_ROW_TILE = 16;
 constexpr int PG_TILE = 128;  // query rows of a tensor-core tile; a large item is two tiles
 
 // Keys per chunk of a small request: 64 up to 2048 keys, where latency counts; then as many as keep what a
-// chunk leaves behind (rows x 528 bytes, written and read again) small against its keys. It goes by the
-// request's own length, so a request is cut alike in every batch. Always a multiple of 64, at most 2048
-// (32 pages: one per lane).
+// chunk leaves behind (rows x 528 bytes, written and read again) small against its keys, which with more than
+// 8 rows begins earlier. It goes by the request's own length and rows, so a request is cut alike in every
+// batch. Always a multiple of 64, at most 2048 (32 pages: one per lane).
 constexpr int PG_CHUNK = 64;
-__host__ __device__ inline int pg_chunk_keys(int len) {
-    if (len <= 2048) return PG_CHUNK;
-    if (len <= 4096) return 128;
+__host__ __device__ inline int pg_chunk_keys(int len, int rows) {
+    if (len <= (rows > 8 ? 512 : 2048)) return PG_CHUNK;
+    if (len <= (rows > 8 ? 1024 : 4096)) return 128;
     return len <= 131072 ? 256 : len <= 524288 ? 1024 : 2048;
 }
-__host__ __device__ inline int pg_chunks(int len) {
-    return len <= 0 ? 0 : (int)(((int64_t)len + pg_chunk_keys(len) - 1) / pg_chunk_keys(len));
+__host__ __device__ inline int pg_chunks(int len, int rows) {
+    return len <= 0 ? 0 : (int)(((int64_t)len + pg_chunk_keys(len, rows) - 1) / pg_chunk_keys(len, rows));
 }
 
 // Tokens of a large item (two tiles of 128 / group tokens), and the items of a request: its keys are split
