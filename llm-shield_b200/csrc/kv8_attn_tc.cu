@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
     int* err = a.b.status;
 
     if (warp >= 12) {
-        reg_dec<32>();
+        reg_dec<48>();
         if (warp < 14) {
             // ------------------------------------------------ issue the products of one tile
             const int x = warp - 12;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             if (!ok && lane == 0) paged_report(err, JV_ERR_DEVICE_TIMEOUT, PS_ATTN_TC + KR_ISSUE);
         }
     } else if (warp >= 8) {
-        reg_dec<96>();
+        reg_dec<128>();
         // ---------------------------------------------------- int8 -> fp16 operands
         const int t = tid - 256, j0 = t & 3, r0 = t >> 2;  // 16 bytes j0 and j0 + 4 of rows r0 + 32 k
         const int32_t* table = a.b.block_table + (int64_t)item.x * a.b.max_blocks;
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             if (n + 1 < blocks) load(vr, v0, v1, 1);
         }
     } else {
-        reg_inc<192>();
+        reg_inc<168>();
         // ---------------------------------------------------- softmax and output, a query row per thread
         const int x = warp >> 2, r = tid & 127;
         const int b0 = it.b0[x], b1 = it.b1[x], nt = it.nt[x], t0 = it.t0[x];
@@ -384,90 +384,110 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             }
             tc_fence_after();
             const float4* sc = scales + ((b - it.lo) & (KT_SLOTS - 1)) * 8;
-            uint32_t v[128];
-            {
-                uint32_t(&v0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[0]);
-                uint32_t(&v1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[32]);
-                uint32_t(&v2)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[64]);
-                uint32_t(&v3)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[96]);
-                tld32(s_col, v0);
-                tld32(s_col + 32u, v1);
-                tld32(s_col + 64u, v2);
-                tld32(s_col + 96u, v3);
-                tld_wait(v0);
-                tld_wait(v1);
-                tld_wait(v2);
-                tld_wait(v3);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_free + 8 * x);  // S(b + 1) may overwrite S(b)
             const int k0 = b * KT_KEYS, vis_hi = hi_key - k0, vis_lo = lo_key - k0;
             const bool all = __all_sync(0xffffffffu, vis_hi >= KT_KEYS && vis_lo <= 0);
-            float bm = -INFINITY;
-            if (!all) {
-                // a block that some row does not see whole: the exponents themselves, masked, in place
+            // The block in two halves of 64 keys, so that a thread holds 64 scores and not 128.
+            uint32_t v[64];
+            auto load = [&](int half) {
+                uint32_t(&v0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[0]);
+                uint32_t(&v1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[32]);
+                tld32(s_col + (uint32_t)(64 * half), v0);
+                tld32(s_col + (uint32_t)(64 * half + 32), v1);
+                tld_wait(v0);
+                tld_wait(v1);
+            };
+            // The half's largest exponent. Where some row does not see the whole block, v becomes the exponents
+            // themselves, masked.
+            auto largest = [&](int half) {
+                float bm = -INFINITY;
+                if (!all) {
 #pragma unroll
-                for (int h = 0; h < 8; h++) {
-                    const float4 s = sc[h];
-                    const float ka = s.x * qs, kb = fmaf(s.x, qb, s.y);
+                    for (int h = 0; h < 4; h++) {
+                        const float4 s = sc[4 * half + h];
+                        const float ka = s.x * qs, kb = fmaf(s.x, qb, s.y);
 #pragma unroll
-                    for (int e = 16 * h; e < 16 * h + 16; e++) {
-                        const float y = fmaf(__uint_as_float(v[e]), ka, kb);
-                        v[e] = __float_as_uint(e < vis_hi && e >= vis_lo ? y : -INFINITY);
-                        bm = fmaxf(bm, __uint_as_float(v[e]));
+                        for (int e = 16 * h; e < 16 * h + 16; e++) {
+                            const float y = fmaf(__uint_as_float(v[e]), ka, kb);
+                            v[e] = __float_as_uint(64 * half + e < vis_hi && 64 * half + e >= vis_lo ? y : -INFINITY);
+                            bm = fmaxf(bm, __uint_as_float(v[e]));
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 4; h++) {
+                        const float4 s = sc[4 * half + h];
+                        // three inputs at a time, in two chains
+                        float g = max3(__uint_as_float(v[16 * h]), __uint_as_float(v[16 * h + 1]), __uint_as_float(v[16 * h + 2]));
+                        float g1 = max3(__uint_as_float(v[16 * h + 3]), __uint_as_float(v[16 * h + 4]), __uint_as_float(v[16 * h + 5]));
+#pragma unroll
+                        for (int e = 16 * h + 6; e < 16 * h + 14; e += 4) {
+                            g = max3(g, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                            g1 = max3(g1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+                        }
+                        g = max3(fmaxf(g, g1), __uint_as_float(v[16 * h + 14]), __uint_as_float(v[16 * h + 15]));
+                        bm = fmaxf(bm, fmaf(g, s.x * qs, fmaf(s.x, qb, s.y)));
                     }
                 }
-            } else {
+                return bm;
+            };
+            // The half's weights as fp16 pairs in v[0..31], and their sum over the values' scales.
+            auto weights = [&](int half, float ref) {
+                float rs = 0.f;
 #pragma unroll
-                for (int h = 0; h < 8; h++) {
-                    const float4 s = sc[h];
-                    // three inputs at a time, in two chains
-                    float g = max3(__uint_as_float(v[16 * h]), __uint_as_float(v[16 * h + 1]), __uint_as_float(v[16 * h + 2]));
-                    float g1 = max3(__uint_as_float(v[16 * h + 3]), __uint_as_float(v[16 * h + 4]), __uint_as_float(v[16 * h + 5]));
+                for (int h = 0; h < 4; h++) {
+                    const float4 s = sc[4 * half + h];
+                    const float ka = all ? s.x * qs : 1.f, kb = (all ? fmaf(s.x, qb, s.y) : 0.f) - ref;
+                    const uint64_t ka2 = pack_f32x2(ka, ka), kb2 = pack_f32x2(kb, kb);
+                    uint64_t g2 = 0;
 #pragma unroll
-                    for (int e = 16 * h + 6; e < 16 * h + 14; e += 4) {
-                        g = max3(g, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-                        g1 = max3(g1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+                    for (int e = 16 * h; e < 16 * h + 16; e += 2) {
+                        const float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), ka2, kb2));
+                        const float w0 = ex2(y.x), w1 = ex2(y.y);
+                        g2 = add_f32x2(g2, pack_f32x2(w0, w1));
+                        const __half2 hp = __floats2half2_rn(w0, w1);
+                        v[e >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
                     }
-                    g = max3(fmaxf(g, g1), __uint_as_float(v[16 * h + 14]), __uint_as_float(v[16 * h + 15]));
-                    bm = fmaxf(bm, fmaf(g, s.x * qs, fmaf(s.x, qb, s.y)));
+                    const float2 gs = unpack_f32x2(g2);
+                    rs = fmaf(gs.x + gs.y, s.z, rs);
                 }
-            }
-            const bool move = bm > m + 8.f;
-            const float mn = move ? bm : m;
-            const float ref = mn == -INFINITY ? 0.f : mn;
-            const float alpha = !move ? 1.f : m == -INFINITY ? 0.f : ex2(m - mn);
-            float rs = 0.f;
+                return rs;
+            };
+            auto store = [&](int half) {
 #pragma unroll
-            for (int h = 0; h < 8; h++) {
-                const float4 s = sc[h];
-                const float ka = all ? s.x * qs : 1.f, kb = (all ? fmaf(s.x, qb, s.y) : 0.f) - ref;
-                const uint64_t ka2 = pack_f32x2(ka, ka), kb2 = pack_f32x2(kb, kb);
-                uint64_t g2 = 0;
-#pragma unroll
-                for (int e = 16 * h; e < 16 * h + 16; e += 2) {
-                    const float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), ka2, kb2));
-                    const float w0 = ex2(y.x), w1 = ex2(y.y);
-                    g2 = add_f32x2(g2, pack_f32x2(w0, w1));
-                    const __half2 hp = __floats2half2_rn(w0, w1);
-                    v[e >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
-                }
-                const float2 gs = unpack_f32x2(g2);
-                const float g = gs.x + gs.y;
-                rs = fmaf(g, s.z, rs);
-            }
-            l = fmaf(l, alpha, rs);
-            m = mn;
+                for (int c = 0; c < 8; c++)
+                    *(uint4*)(sm + (5 + x) * KT_TILE + tile_off(r, 8 * half + c)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+            };
+            load(0);
+            float bm = largest(0);
+            float mn = bm > m + 8.f ? bm : m;
+            float rs = weights(0, mn == -INFINITY ? 0.f : mn);
             // W is free, and O holds every block before b, once W V(b - 1) is done
             if (b > b0 && !warp_wait(o_done + 8 * x, (uint32_t)((b - 1 - b0) & 1))) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < 16; c++)
-                *(uint4*)(sm + (5 + x) * KT_TILE + tile_off(r, c)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+            store(0);
+            load(1);
+            bm = largest(1);
+            if (__any_sync(0xffffffffu, bm > mn + 8.f)) {
+                // the second half moves a row's reference: the first again, at the new one
+                mn = bm > mn + 8.f ? bm : mn;
+                load(0);
+                largest(0);
+                rs = weights(0, mn == -INFINITY ? 0.f : mn);
+                store(0);
+                load(1);
+                largest(1);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_free + 8 * x);  // S(b + 1) may overwrite S(b)
+            rs += weights(1, mn == -INFINITY ? 0.f : mn);
+            store(1);
+            const float alpha = mn == m ? 1.f : m == -INFINITY ? 0.f : ex2(m - mn);
+            l = fmaf(l, alpha, rs);
+            m = mn;
             // O *= alpha where a row's reference moved
             if (b > b0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
