@@ -481,10 +481,11 @@ __global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
     pdl_wait();
     const int row = blockIdx.x, request = blockIdx.y, kvh = blockIdx.z;
     RequestRows rr;
+    const int first = a.v.first[request];  // asked for together with the rows
     if (!request_rows(a.b, request, rr)) return;
     const int n_rows = rr.n_new * a.b.group, chunks = pg_chunks(rr.len, n_rows);
     if (n_rows > PG_SMALL_ROWS || row >= n_rows || chunks < 2) return;
-    const int first = a.v.first[request], item0 = first + row / PG_ROW_TILE * chunks;
+    const int item0 = first + row / PG_ROW_TILE * chunks;
     if (first < 0 || item0 + chunks > a.v.small_cap) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t p0 = ((int64_t)item0 * a.c.kv_heads + kvh) * a.rows + row % PG_ROW_TILE, step = (int64_t)a.c.kv_heads * a.rows;

@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
                         }
                         *(uint4*)(dst + 8 * c) = make_uint4(y[0], y[1], y[2], y[3]);
                     }
-                } else {
+                } else if (any) {  // without a block, the reference of -infinity below says so
                     float4* dst = (float4*)(a.large_o + part * PG_DIM + 32 * h);
 #pragma unroll
                     for (int c = 0; c < 8; c++)
@@ -569,7 +569,7 @@ template <class T>
 __device__ __forceinline__ void join_row(const AttnKArgs& a, int4 item, int kvh, int row, int lane) {
     const int splits = item.w & 255, place = item.w >> 8;
     RequestRows rr;
-    if (splits > 16 || place < 0 || place + splits > a.v.split_cap || !request_rows(a.b, item.x, rr)) return;
+    if (splits > PG_SPLIT_ITEMS || place < 0 || place + splits > a.v.split_cap || !request_rows(a.b, item.x, rr)) return;
     const int group = a.b.group, tt = PG_TILE / group, x = row / PG_TILE, r = row % PG_TILE, tok = r / group;
     const int t = item.y * 2 * tt + x * tt + tok;
     if (tok >= tt || t < 0 || t >= rr.n_new) return;
@@ -585,8 +585,9 @@ __device__ __forceinline__ void join_row(const AttnKArgs& a, int4 item, int kvh,
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int s = 0; s < splits; s++) {
-        const float4 y = *(const float4*)(a.large_o + (p0 + s * step) * PG_DIM + 4 * lane);
         const float g = __shfl_sync(0xffffffffu, f, s);
+        if (g == 0.f) continue;  // also the splits without a block, which left no values
+        const float4 y = *(const float4*)(a.large_o + (p0 + s * step) * PG_DIM + 4 * lane);
         o.x = fmaf(y.x, g, o.x), o.y = fmaf(y.y, g, o.y), o.z = fmaf(y.z, g, o.z), o.w = fmaf(y.w, g, o.w);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;

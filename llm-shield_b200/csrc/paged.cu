@@ -87,8 +87,9 @@ PlanView plan_view(const jv_paged_batch& b) {
     const int64_t per = most <= 4096 ? std::min<int64_t>(32, (most + PG_CHUNK - 1) / PG_CHUNK) : std::max<int64_t>(512, (most + 2047) / 2048);
     v.small_cap = std::min(R + std::min(b.max_keys / PG_CHUNK, 32 * R + b.max_keys / 128), R * per) * tiles;
     const int64_t large = (int64_t)b.max_new * b.group > PG_SMALL_ROWS ? std::min<int64_t>(R, T * b.group / (PG_SMALL_ROWS + 1)) : 0;
-    // at most 16 / pairs splits of each of up to 7 pairs, and a split has at least 1024 keys but for a request's last
-    v.split_cap = std::min(16 * large, 7 * (large + b.max_keys / 1024));
+    // at most PG_SPLIT_ITEMS / pairs splits of each of up to a quarter as many pairs, and a split has at least 1024
+    // keys but for a request's last
+    v.split_cap = std::min(PG_SPLIT_ITEMS * large, PG_SPLIT_ITEMS / 4 * (large + b.max_keys / 1024));
     v.large_cap = large ? v.split_cap + large + T / pg_pair_tokens(b.group) : 0;
     v.unit_cap = std::min<int64_t>(T, T / PG_BLOCK + 2 * R);
     uint8_t* p = (uint8_t*)b.work;

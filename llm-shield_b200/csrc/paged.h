@@ -35,13 +35,17 @@ __host__ __device__ inline int pg_chunks(int len, int rows) {
 }
 
 // Tokens of a large item (two tiles of 128 / group tokens), and the items of a request: its keys are split
-// too, in up to 16 parts of at least 1024 keys, where it has few tiles. By the request's own sizes again.
+// too, in parts of at least 1024 keys, where it has at most 4 pairs of tiles: up to 16 items. (From 5 pairs on the
+// parts' results, 128 KB each, cost more than the balance gives: five chunks of 100 to 1500 tokens in a window
+// take 285 us without them, 317 with up to 16 items for up to 8 pairs, 461 with 32.) By the request's own sizes
+// again.
+constexpr int PG_SPLIT_ITEMS = 16;  // a split of a pair is joined by a lane each
 __host__ __device__ inline int pg_pair_tokens(int group) { return 2 * (PG_TILE / group); }
 __host__ __device__ inline int pg_pairs(int n_new, int group) { return (n_new + pg_pair_tokens(group) - 1) / pg_pair_tokens(group); }
 __host__ __device__ inline int pg_splits(int len, int pairs) {
-    if (pairs >= 8) return 1;
+    if (pairs > PG_SPLIT_ITEMS / 4) return 1;
     const int blocks = (int)(((int64_t)len + 127) / 128), most = (blocks + 7) / 8;
-    return most < 1 ? 1 : most < 16 / pairs ? most : 16 / pairs;
+    return most < 1 ? 1 : most < PG_SPLIT_ITEMS / pairs ? most : PG_SPLIT_ITEMS / pairs;
 }
 
 // A plan's work lists, in jv_paged_batch.work.
