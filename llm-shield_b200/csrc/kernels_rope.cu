@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope(RopeKArgs a, int per_cta) {
 // "piece" is V consecutive elements of adjacent pairs, or both halves of V half-split pairs, or, in a second
 // sweep, V elements behind rotary_dim; a power of two of lanes takes a head's pieces, so that every lane of a
 // warp has the same kind. Bound by HBM: four (token, head) rows per thread in flight, the first four before
-// the angles are worked out. 8191 tokens x 40 heads of 128 in bf16, half of them turned: see the case table.
+// the angles are worked out. 8191 tokens x 40 heads of 128 in bf16, half of each turned: 35 us, 74 % of the
+// measured copy rate.
 template <class T>
 union Vec {
     uint4 raw;
@@ -371,7 +372,8 @@ __device__ __forceinline__ uint32_t quantise4(const float (&x)[4], float inv, bo
 
 // One CTA: a 16-token block that the step writes to, a slice of its heads; one warp a head at a time
 // (a lane holds 4 dimensions of the 16 tokens, so a block's largest magnitude is one register
-// reduction and one shuffle tree).
+// reduction over the lanes). Latency-bound: 16 rows of a head are in flight per warp, 16 warps per SM
+// (5,500 tokens x 8 KV heads in bf16: 15 us, floor 5.3).
 template <class T, class TQ, bool VEC, bool ROPE>
 __global__ void __launch_bounds__(RP_THREADS, 2) k_kv8_append(AppendArgs a) {
     __shared__ float2 cs[PG_BLOCK][64];

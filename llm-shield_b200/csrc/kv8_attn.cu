@@ -4,14 +4,14 @@
 // are the scales of key j's block of 16. The scales never touch the matrices: with
 //   e_j = scale ks(j) (q . kint_j) + log2 vs(j)   (in log2 units),   w_j = 2^(e_j - M),   M >= max e_j - 8
 // the output is  sum_j w_j vint_j / sum_j (w_j / vs(j)),  so the products run on exact integers (an
-// int8 is exact in fp16), w_j <= 2^8 is the only rounded operand (fp16, half a step 2^-12), and sums, M
+// int8 is exact in fp16), w_j <= 2^8 is the only rounded operand (fp16, half a step 2^-11), and sums, M
 // and the softmax denominator are fp32. bf16 queries are taken to fp16 by a power of two per row.
 //
 // Here: the requests of few query rows, whose time is the cache's bytes. (kv8_attn_tc.cu has the others.)
 // The products are mma.sync m16n8k16 with the keys on the 16-row side and the query rows (new token x
 // head of the group) on the 8-column side: S^T = K Q^T, O^T = V^T P^T. The order of the 128
 // dimensions inside a product is free, so a lane loads 16 consecutive int8 of its rows straight from
-// the cache into fragments; S^T becomes the operand P^T by one movmatrix per 8 x 8 block.
+// the cache's rows into fragments; S^T becomes the operand P^T by one movmatrix per 8 x 8 block.
 #include <atomic>
 #include <cmath>
 #include <string>
@@ -103,9 +103,10 @@ __device__ __forceinline__ void store_row(const AttnKArgs& a, int start, int kvh
 // that the fragment loads below meet no bank twice); it refills a stage as soon as it has used it, with its
 // next keys or already with the first of its next item. Nothing joins the warps: a chunk's result goes to
 // the workspace (k_kv8_join), or out when the request has one chunk. Bound by HBM: 12 warps keep 96 KB per SM
-// in flight; a 16-key tile costs about 250 instructions, a third of the issue slots at the HBM rate.
-// With two 8-row tiles per warp (NT = 2) the registers leave 8 warps per SM, with a third stage each. (Query
-// fragments in shared memory instead, for 12 warps: 108 against 88 us for 24 requests of 2 to 6 new tokens.)
+// in flight; a 16-key tile costs about 360 instructions (64 requests of 300 to 8000 keys: 98 us, 5.5 TB/s).
+// With two 8-row tiles per warp (NT = 2) the registers leave 8 warps per SM, with a third stage each, and latency
+// is what bounds it (24 requests of 2 to 6 new tokens: 82 us; query fragments in shared memory, for 12 warps: 108;
+// three 8-row tiles: 92).
 constexpr int KS_WARPS = 4;
 template <int NT>
 struct Ks {

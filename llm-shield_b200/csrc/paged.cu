@@ -419,7 +419,7 @@ int jv_paged_plan(const jv_paged_batch* batch, const int32_t* cached, const int3
         OnDeviceOf dev(batch->work);
         PlanArgs a{*batch, plan_view(*batch), cached, new_tokens, free_pages, n_free, n_free_out};
         // A CTA of few warps for few requests. It fills the arrays too where a warp per request gets
-        // through them in less than a second launch costs (16 requests of one token: 3.9 us in one launch).
+        // through them in less than a second launch costs (16 requests of one token: 6.8 us in one launch).
         const bool fill = batch->requests <= PLAN_FILL_REQUESTS && batch->max_new <= 256 && batch->max_tokens <= 4096;
         const int threads = batch->requests <= 8 ? 256 : PLAN_THREADS;
         launch_pdl(k_plan, dim3(1), dim3(threads), 0, (cudaStream_t)stream, a, fill);

@@ -90,7 +90,7 @@ int paged_api(F&& f) {
 // Sites of the status word (word 1).
 enum PagedSite : int {
     PS_PLAN_LENGTH = 96, PS_PLAN_TOKENS = 97, PS_PLAN_KEYS = 98, PS_PLAN_FREE = 99, PS_PLAN_PAGE = 100,
-    PS_APPEND_PAGE = 101, PS_APPEND_VALUE = 102, PS_READ_SLOT = 103, PS_READ_VALUE = 104, PS_ATTN_REQUEST = 105,
+    PS_APPEND_PAGE = 101, PS_APPEND_VALUE = 102, PS_READ_SLOT = 103, PS_READ_VALUE = 104,
     PS_ATTN_PAGE = 106, PS_ROPE_VALUE = 107, PS_ATTN_WAIT = 108, PS_ATTN_TC = 112 /* + role */
 };
 
