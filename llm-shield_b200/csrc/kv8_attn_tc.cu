@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
     it.tt = PG_TILE / group;
     const int total_blocks = (int)(((int64_t)it.rr.len + KT_KEYS - 1) / KT_KEYS);
     const int per = splits > 0 ? (total_blocks + splits - 1) / splits : 0;
-    if (item.y < 0 || item.z < 0 || item.z >= splits || (splits > 1 && (place < 0 || place + item.z >= a.v.split_cap)) || (int64_t)item.y * 2 * it.tt >= it.rr.n_new) return;
+    if (item.y < 0 || item.z < 0 || item.z >= splits || (splits > 1 && (place < 0 || place >= a.v.split_cap)) || (int64_t)item.y * 2 * it.tt >= it.rr.n_new) return;
     const int s0 = min(item.z * per, total_blocks), s1 = min(s0 + per, total_blocks);
     it.lo = 1 << 30, it.hi = 0;
 #pragma unroll

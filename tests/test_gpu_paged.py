@@ -699,3 +699,45 @@ def test_device_memory_is_required():
     h = paged.heads(k.data_ptr(), 1, 128, 128)
     with pytest.raises(ArgumentError):
         paged.kv8_append(c, s.batch, "f32", h, h)
+
+
+# ------------------------------------------------------------------------------------------ at the edges
+
+
+def filled(requests, g, group, first, new, dtype, seed, **more):
+    """A server whose requests hold `first` tokens and are planned and appended for `new` more; queries for them."""
+    most = max(max(first), max(new))
+    blocks = -(-max(a + b for a, b in zip(first, new)) // 64)
+    s = Server(requests, g, group, requests * blocks, most, max(sum(first), sum(new)), blocks, seed=seed, **more)
+    gen = torch.Generator("cuda").manual_seed(seed)
+    for step in (first, new):
+        s.plan(step)
+        kv = torch.randn(max(sum(step), 1), 2, g, 128, generator=gen, device="cuda")
+        s.append(kv[:, 0], kv[:, 1], "f32")
+    q = torch.randn(sum(new), g * group, 128, generator=gen, device="cuda").to(TYPE[dtype])
+    return s, q
+
+
+@pytest.mark.parametrize("g,group,first,new", [
+    (1, 2, [140001], [1]), (1, 2, [140001], [2]), (1, 2, [530000], [1]), (1, 2, [140001], [40]),
+    (2, 4, [20000, 9000, 5000, 3000, 70], [40, 64, 128, 33, 50]), (1, 4, [9000, 9001, 30000], [200, 33, 64]),
+    (3, 1, [17000, 6000], [300, 512]), (1, 8, [16000, 16000, 2000, 16000], [40, 3, 40, 1])])
+def test_long_contexts_and_their_splits(g, group, first, new):
+    """The longer chunks (1024 and 2048 keys), up to 16 splits of several requests, and their joins, against 64
+    bits on the GPU."""
+    s, q = filled(len(new), g, group, first, new, "f16", 6)
+    q *= 3
+    got = s.attend(q, "f16")
+    at = 0
+    for r, (n, m) in enumerate(zip(first, new)):
+        pages = s.table[r, :-(-(n + m) // 64)].long()
+        x = s.data.view(s.pages, g, 2, 64, 128)[pages].double() * s.scales.view(s.pages, g, 2, 4)[pages].double().repeat_interleave(16, -1)[..., None]
+        hide = torch.arange(n + m, device="cuda") > torch.arange(n, n + m, device="cuda")[:, None]
+        for h in range(g * group):
+            k, v = (x[:, h // group, c].reshape(-1, 128)[:n + m] for c in (0, 1))
+            p = torch.softmax((q[at:at + m, h].double() @ k.T * 128 ** -0.5).masked_fill(hide, -math.inf), -1)
+            want, mag = p @ v, p @ v.abs()
+            tol = HALF["f16"] * want.abs() + (2.0 ** -11 + 2.0 ** -13) * mag + (n + m) * 2.0 ** -25 * v.abs().max() + 2.0 ** -25
+            assert ((got[at:at + m, h].double() - want).abs() <= tol).all(), (r, h)
+        at += m
+    assert s.status.tolist() == [0, 0]
