@@ -25,6 +25,11 @@ __device__ __forceinline__ float2 rope_angle(double turns, int pos, float mscale
     return make_float2(c * mscale, s * mscale);
 }
 
+// The query temperature; a position below 0 has none.
+__device__ __forceinline__ float temperature_at(const jv_rope_spec& s, int pos) {
+    return pos < 0 ? 1.f : rope_temperature(pos, s.temperature_ctx, s.temperature_scale);
+}
+
 template <class T>
 __device__ __forceinline__ float ld1(const T* p);
 template <>
@@ -122,7 +127,7 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope(RopeKArgs a, int per_cta) {
         cs[t][f] = rope_angle(a.spec.turns[f], a.positions[t0 + t], a.spec.mscale);
     }
     if (threadIdx.x < nt)
-        temp[threadIdx.x] = rope_temperature(a.positions[t0 + threadIdx.x], a.spec.temperature_ctx, a.spec.temperature_scale);
+        temp[threadIdx.x] = temperature_at(a.spec, a.positions[t0 + threadIdx.x]);
     __syncthreads();
     const int h0 = blockIdx.y * per_cta, nh = min(per_cta, a.n_heads - h0), pairs = a.dim >> 1;
     for (int i = threadIdx.x; i < nt * nh * pairs; i += RP_THREADS) {
@@ -258,7 +263,7 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope_vec(RopeKArgs a, int per_ct
         cs[ti][f] = rope_angle(a.spec.turns[f], a.positions[t0 + ti], a.spec.mscale);
     }
     if (threadIdx.x < nt)
-        temp[threadIdx.x] = rope_temperature(a.positions[t0 + threadIdx.x], a.spec.temperature_ctx, a.spec.temperature_scale);
+        temp[threadIdx.x] = temperature_at(a.spec, a.positions[t0 + threadIdx.x]);
     __syncthreads();
     while (tt[0] != 255) {
 #pragma unroll
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(RP_THREADS, 2) k_kv8_append(AppendArgs a) {
             if (t >= lo && t < hi) cs[t][f] = rope_angle(a.spec.turns[f], p0 + t, a.spec.mscale);
         }
         if (threadIdx.x < PG_BLOCK)
-            temp[threadIdx.x] = rope_temperature(p0 + threadIdx.x, a.spec.temperature_ctx, a.spec.temperature_scale);
+            temp[threadIdx.x] = temperature_at(a.spec, p0 + threadIdx.x);
         __syncthreads();
     }
     const int lane = threadIdx.x & 31, g = a.c.kv_heads;

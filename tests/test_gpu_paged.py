@@ -741,3 +741,18 @@ def test_long_contexts_and_their_splits(g, group, first, new):
             assert ((got[at:at + m, h].double() - want).abs() <= tol).all(), (r, h)
         at += m
     assert s.status.tolist() == [0, 0]
+
+
+def test_rope_at_positions_below_zero():
+    """A position below 0 turns backwards and has no query temperature."""
+    from jevstral_b200 import paged
+
+    spec = paged.rope_spec("half", 128, 1e4, temperature_scale=0.1, temperature_context=4)
+    x = torch.randn(3, 2, 128, device="cuda")
+    y = torch.empty_like(x)
+    pos = torch.tensor([-1, -100, 3], dtype=torch.int32, device="cuda")
+    paged.rope(spec, "f32", pos.data_ptr(), 3, 128, paged.heads(x.data_ptr(), 2, 256, 128, y.data_ptr(), temperature=True))
+    torch.cuda.synchronize()
+    want = rope64(x.double().cpu().numpy(), pos.cpu().numpy(), spec)
+    # two products of factors off by at most 2 steps of 2^-23 each, and their sum: 6 steps of 2^-23 at |a| + |b| < 10
+    assert np.abs(y.double().cpu().numpy() - want).max() < 6 * 2.0 ** -23 * 10
