@@ -267,7 +267,8 @@ int64_t jv_paged_work_bytes(const jv_paged_batch* batch);
  * taken from the end of free_pages[*n_free] (in request order, then block order: free_pages[*n_free
  * - 1] first) and *n_free_out becomes the count left. Every array of the batch is written. cached may
  * be lengths and n_free_out may be n_free, for a step that continues the last. Requests may share
- * pages that are full; a page that a request writes to must be its own.
+ * pages that are full; a page that a request writes to must be its own, and free_pages must not name a
+ * page twice or one in use.
  * If a bound of the batch is exceeded (JV_ERR_RANGE), free pages run out (JV_ERR_OOM) or a free page
  * is not in the cache (JV_ERR_RANGE), no page is taken, lengths become cached and starts 0: the
  * operators after it then do nothing. */
@@ -306,7 +307,8 @@ typedef struct jv_heads {
 } jv_heads;
 
 /* Rotates x[0..n) (queries and keys, n = 1 or 2) at positions[tokens]; the elements from rotary_dim on
- * are copied. head_dim: even, up to 256, at least rotary_dim. tokens == 0 does nothing. */
+ * are copied. head_dim: even, up to 256, at least rotary_dim. tokens == 0 does nothing. A result outside
+ * the type's range becomes an infinity. */
 int jv_rope(const jv_rope_spec* spec, int32_t type, const int32_t* positions, int32_t tokens, int32_t head_dim,
             const jv_heads* x, int32_t n, void* stream);
 

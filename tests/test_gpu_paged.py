@@ -718,6 +718,45 @@ def filled(requests, g, group, first, new, dtype, seed, **more):
     return s, q
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new", [[3, 1], [60, 33]])
+def test_a_row_that_is_not_finite_stays_its_own(dtype, new):
+    s, q = filled(2, 2, 4, [300, 90], new, dtype, 3)
+    want = s.attend(q, dtype)
+    for bad in (math.nan, math.inf):
+        p = q.clone()
+        p[1, 3, 17] = bad
+        got = s.attend(p, dtype)
+        torch.cuda.synchronize()
+        assert not torch.isfinite(got[1, 3]).all()
+        got[1, 3] = want[1, 3]
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 2.0])
+@pytest.mark.parametrize("new", [[2], [50]])
+def test_scales_of_any_sign(scale, new):
+    s, q = filled(1, 2, 4, [260], new, "f16", 4)
+    out = torch.empty_like(q)
+    h = s.p.heads(q.data_ptr(), 8, q.stride(0), q.stride(1), out.data_ptr())
+    s.p.kv8_attention(s.cache, s.batch, "f16", h, scale, 0, s.ws.data_ptr(), s.ws_bytes)
+    torch.cuda.synchronize()
+    compare(out, q, s, "f16", new, scale, 0)
+
+
+@pytest.mark.parametrize("new", [[2, 1], [40, 70]])
+def test_attention_in_place_and_repeated(new):
+    """The output over the queries, and the same call again on an output that holds the last: the same bits."""
+    s, q = filled(2, 2, 4, [700, 100], new, "bf16", 5)
+    want = s.attend(q, "bf16")
+    for _ in range(3):
+        assert torch.equal(s.attend(q, "bf16"), want)
+    p = q.clone()
+    s.attend(p, "bf16", out=p)
+    torch.cuda.synchronize()
+    assert torch.equal(p, want)
+
+
 @pytest.mark.parametrize("g,group,first,new", [
     (1, 2, [140001], [1]), (1, 2, [140001], [2]), (1, 2, [530000], [1]), (1, 2, [140001], [40]),
     (2, 4, [20000, 9000, 5000, 3000, 70], [40, 64, 128, 33, 50]), (1, 4, [9000, 9001, 30000], [200, 33, 64]),
@@ -743,6 +782,13 @@ def test_long_contexts_and_their_splits(g, group, first, new):
     assert s.status.tolist() == [0, 0]
 
 
+def test_many_kv_heads_and_one_query_head_each():
+    s, q = filled(2, 40, 1, [100, 5], [1, 40], "bf16", 7)
+    got = s.attend(q, "bf16")
+    torch.cuda.synchronize()
+    compare(got, q, s, "bf16", [1, 40], 128 ** -0.5, 0)
+
+
 def test_rope_at_positions_below_zero():
     """A position below 0 turns backwards and has no query temperature."""
     from jevstral_b200 import paged
@@ -756,3 +802,51 @@ def test_rope_at_positions_below_zero():
     want = rope64(x.double().cpu().numpy(), pos.cpu().numpy(), spec)
     # two products of factors off by at most 2 steps of 2^-23 each, and their sum: 6 steps of 2^-23 at |a| + |b| < 10
     assert np.abs(y.double().cpu().numpy() - want).max() < 6 * 2.0 ** -23 * 10
+
+
+def test_the_first_calls_of_a_process_can_be_captured():
+    """plan, append and attention of both kinds captured in a fresh process before any of them has run."""
+    import subprocess
+    import sys
+
+    code = """
+import sys
+sys.path[:0] = ['llm-shield_b200', 'tests', '.']
+import torch
+import test_gpu_paged as t
+s = t.Server(2, 2, 4, 20, 60, 120, 8)
+kv = torch.randn(61, 2, 2, 128, device='cuda')
+q = torch.randn(61, 8, 128, device='cuda').half()
+out = torch.zeros_like(q)
+new = torch.tensor([60, 1], dtype=torch.int32, device='cuda')
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    st = torch.cuda.current_stream().cuda_stream
+    s.p.plan(s.batch, s.lengths.data_ptr(), new.data_ptr(), s.free.data_ptr(), s.n_free.data_ptr(), s.n_free.data_ptr(), st)
+    s.append(kv[:, 0], kv[:, 1], 'f32', stream=st)
+    s.attend(q, 'f16', out=out, stream=st)
+for _ in range(3):
+    g.replay()
+torch.cuda.synchronize()
+assert s.status.tolist() == [0, 0] and s.lengths.tolist() == [180, 3]
+t.compare(out, q, s, 'f16', [60, 1], 128 ** -0.5, 0)
+print('captured')
+"""
+    from conftest import REPO
+
+    r = subprocess.run([sys.executable, "-c", code], cwd=str(REPO), capture_output=True, text=True, timeout=300)
+    assert "captured" in r.stdout, (r.stdout[-1000:], r.stderr[-3000:])
+
+
+def test_wrong_devices_and_pointers_are_refused_before_a_launch():
+    s = Server(1, 1, 4, 2, 4, 4, 2)
+    before = __import__("jevstral_b200").kernel_launches()
+    host = torch.zeros(64)
+    from jevstral_b200 import paged
+    from jevstral_b200._lib import ArgumentError
+
+    with pytest.raises(ArgumentError):
+        paged.rope(paged.rope_spec("half", 64, 1e4), "f32", s.positions.data_ptr(), 1, 64,
+                   paged.heads(host.data_ptr(), 1, 64, 64, host.data_ptr()))
+    assert __import__("jevstral_b200").kernel_launches() == before
