@@ -1434,16 +1434,17 @@ void rc_check(int rc) {
     if (rc != JV_OK) throw Error(rc, g_last_error);
 }
 
+// The host's lengths and free list to the device. A block table needs none: the plan writes the entries of new
+// blocks, and those of the blocks below a request's length are what earlier plans wrote. The status goes with it:
+// a pass that failed may have left one.
 void server_upload(jv_server* v) {
-    std::vector<int32_t> t((size_t)v->max_requests * v->max_blocks, 0);
-    for (int r = 0; r < v->max_requests; r++) std::copy(v->table[r].begin(), v->table[r].end(), t.begin() + (size_t)r * v->max_blocks);
     const int32_t n_free = (int32_t)v->free_pages.size();
     cudaStream_t s = v->x->stream;
-    JV_CUDA(cudaMemcpyAsync(v->d_table.p, t.data(), t.size() * 4, cudaMemcpyHostToDevice, s));
     JV_CUDA(cudaMemcpyAsync(v->d_lengths.p, v->lengths.data(), v->lengths.size() * 4, cudaMemcpyHostToDevice, s));
     if (n_free > 0) JV_CUDA(cudaMemcpyAsync(v->d_free.p, v->free_pages.data(), (size_t)n_free * 4, cudaMemcpyHostToDevice, s));
     JV_CUDA(cudaMemcpyAsync(v->d_counts.p + v->max_requests, &n_free, 4, cudaMemcpyHostToDevice, s));
-    JV_CUDA(cudaStreamSynchronize(s));  // the host vectors go
+    JV_CUDA(cudaMemsetAsync(v->d_status.p, 0, 2 * sizeof(int32_t), s));
+    JV_CUDA(cudaStreamSynchronize(s));  // the host's copies may change
     v->dirty = false;
 }
 
@@ -1481,6 +1482,7 @@ void server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, 
     const int hidden = c.hidden, qdim = c.heads * c.head_dim, kvdim = c.kv_heads * c.head_dim, qkvn = qdim + 2 * kvdim, ff = c.ff;
     const int tpad = gemm_tpad_for(n);
     cudaStream_t s = x->stream;
+    if (v->dirty) server_upload(v);  // and nothing of a failed pass is under way any more
     // one upload: tokens, outputs, rows, counts
     const size_t words = (size_t)n + n_out + n_rows + v->max_requests;
     int32_t* hin = x->h_in.get(words);
@@ -1497,7 +1499,6 @@ void server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, 
     __half* attn = v->attn.get((size_t)n * qdim);
     __half* ctx16 = x->ctx16.get((size_t)tpad * qdim);
     __half* xf = x->xs_ff.get((size_t)tpad * ff);
-    if (v->dirty) server_upload(v);
     v->dirty = true;  // until the pass has gone through
     JV_CUDA(cudaMemcpyAsync(din, hin, 4 * words, cudaMemcpyHostToDevice, s));
     rc_check(jv_paged_plan(&v->batch, v->d_lengths.p, din + n + n_out + n_rows, v->d_free.p, v->d_counts.p + v->max_requests,
@@ -1535,14 +1536,11 @@ void server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, 
     int32_t status[2] = {0, 0};
     JV_CUDA(cudaMemcpyAsync(status, v->d_status.p, sizeof status, cudaMemcpyDeviceToHost, s));
     sync_check(x);
-    if (status[0] != 0) {
-        JV_CUDA(cudaMemsetAsync(v->d_status.p, 0, sizeof status, s));
-        JV_CUDA(cudaStreamSynchronize(s));
+    if (status[0] != 0)
         throw Error(status[0], status[0] == JV_ERR_NUMERIC
                                    ? "a rotated query, or a key or value for the 8-bit cache, is not in the fp16 range or not a number"
                                : status[0] == JV_ERR_DEVICE_TIMEOUT ? "a device-side wait timed out (attention over the 8-bit cache)"
                                                                     : "a paged-batch operator refused the pass (site " + std::to_string(status[1]) + ")");
-    }
     // the pass went through: the device's lengths, tables and free list are the host's
     for (int r = 0; r < v->max_requests; r++) {
         v->lengths[r] += counts[r];
@@ -1956,7 +1954,6 @@ int jv_server_create(jv_model* m, int32_t max_requests, int32_t max_context, int
         v->max_tokens = max_tokens, v->pages = pages > 0 ? pages : (int)all;
         v->lengths.assign(max_requests, 0);
         v->table.resize(max_requests);
-        for (int i = v->pages - 1; i >= 0; i--) v->free_pages.push_back(i);
         // the model's own frequencies (fp32, YaRN mixed in when active), in turns
         v->rope.layout = JV_ROPE_ADJACENT;
         v->rope.rotary_dim = c.rope_dim;
@@ -1994,6 +1991,8 @@ int jv_server_create(jv_model* m, int32_t max_requests, int32_t max_context, int
         v->ws.get((size_t)v->ws_bytes);
         uint8_t* data = v->data.get((size_t)v->pages * v->page_bytes);
         float* scales = v->scales.get((size_t)v->pages * v->scale_stride);
+        v->free_pages.resize(v->pages);
+        for (int i = 0; i < v->pages; i++) v->free_pages[i] = v->pages - 1 - i;
         for (int l = 0; l < c.layers; l++)
             v->layers.push_back({data + (int64_t)l * c.kv_heads * 2 * PG_PLANE, scales + (int64_t)l * c.kv_heads * 8, v->page_bytes,
                                  v->scale_stride, v->pages, c.kv_heads});

@@ -106,3 +106,28 @@ def test_a_value_outside_fp16_is_reported(model_factory):
             with pytest.raises(jv.NumericError):
                 s.forward({0: toks(9, 1)}, ROWS)
             assert s.length(0) == 0
+
+
+def test_a_pass_after_one_that_failed(model_factory, tmp_path):
+    """One token's embedding is infinite: its pass fails on the device, and the next one, without it, gives what
+    it gives on a server that saw no failure."""
+    import gguf
+
+    path = tmp_path / "bad.gguf"
+    raw = bytearray(open(model_factory(SMALL_CFG, "Q8_0"), "rb").read())
+    t = next(t for t in gguf.GGUFReader(model_factory(SMALL_CFG, "Q8_0")).tensors if t.name == "token_embd.weight")
+    row = SMALL_CFG.hidden // 32 * 34
+    for b in range(t.data_offset + 2000 * row, t.data_offset + 2001 * row, 34):
+        raw[b:b + 2] = b"\x00\x7c"  # the block's fp16 scale
+    path.write_bytes(raw)
+    with jv.Model(path, kv_pool_mb=64) as m, jv.Server(m, 2, 200, 150) as s, jv.Server(m, 2, 200, 150) as other:
+        p = {0: toks(32, 1), 1: toks(16, 2)}
+        for x in (s, other):
+            x.forward(p, ROWS)
+        for bad in ({0: [2000] * 3, 1: [1001]}, {0: [2000]}):
+            with pytest.raises(jv.NumericError):
+                s.forward(bad, ROWS)
+            assert (s.length(0), s.length(1)) == (32, 16)
+        for step in ({0: toks(70, 3), 1: [1500]}, {0: [1501], 1: [1502]}):
+            a, b = s.forward(step, ROWS), other.forward(step, ROWS)
+            assert all(np.array_equal(a[r], b[r]) for r in step)
