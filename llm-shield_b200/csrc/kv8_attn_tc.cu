@@ -10,8 +10,8 @@
 // TMEM: O_A, O_B, S_A, S_B, 128 columns each. A softmax hands its S columns back as soon as it has them in
 // registers, so the next block's S runs under its exponentials, and each tile has its own W: the softmaxes
 // never wait for the tensor pipe but at the start. (W over S in TMEM, which saves the shared memory, ran 213 to
-// 230 us where this takes 195: S, softmax and W V one after the other.) A prompt of 4095 tokens, 32 / 8 heads: 704
-// TFLOP/s of visible work, about 5,200 cycles a block of the two tiles. What bounds it is the chain of the softmax
+// 230 us where this took 195: S, softmax and W V one after the other.) A prompt of 4095 tokens, 32 / 8 heads: 182 us,
+// 752 TFLOP/s of visible work, about 4,700 cycles a block of the two tiles. What bounds it is the chain of the softmax
 // (scores out of TMEM, largest, exponentials, weights to shared memory) at two warps per scheduler: the exponential
 // unit is busy for 2,048 of them, the tensor pipe for 2,048, shared memory for about 3,200.
 // Warps 0-3 and 4-7: the softmax and output of tiles A and B. Warps 8-11: convert the cache's int8 to fp16
@@ -129,11 +129,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
     pdl_wait();
     pdl_launch_dependents();
     const int kvh_n = a.c.kv_heads, kvh = blockIdx.x % kvh_n, index = blockIdx.x / kvh_n;
+    // in the lists' bounds, as the grid is; all at once, since every load that waits for another costs 700 cycles
+    const int4 item = a.v.large_items[index], rows = a.v.large_rows[index];
     if (index >= a.v.head[1]) return;
-    const int4 item = a.v.large_items[index];
     const int group = a.b.group, splits = item.w & 255, place = item.w >> 8;
     KtItem it;
-    if (!request_rows(a.b, item.x, it.rr)) return;
+    it.rr.start = rows.x, it.rr.n_new = rows.y, it.rr.len = rows.z;
+    if (item.x < 0 || item.x >= a.b.requests || !rows_in_bounds(a.b, rows.x, rows.y, rows.z)) return;
     it.tt = PG_TILE / group;
     const int total_blocks = (int)(((int64_t)it.rr.len + KT_KEYS - 1) / KT_KEYS);
     const int per = splits > 0 ? (total_blocks + splits - 1) / splits : 0;
@@ -152,6 +154,22 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
     }
     if (it.lo > it.hi) it.lo = it.hi;
 
+    // The first loads from the pages' table, on their way while the CTA sets up.
+    const int32_t* table = a.b.block_table + (int64_t)item.x * a.b.max_blocks;
+    const int pages = (int)(((int64_t)it.rr.len + PG_TOKENS - 1) / PG_TOKENS);
+    // the two pages of a block; -1 where the request has none
+    auto page_of = [&](int b, int h) {
+        const int p = 2 * b + h;
+        if (b >= it.hi || p >= pages) return -1;
+        const int id = table[p];
+        if ((unsigned)id >= (unsigned)a.c.pages) {
+            if (lane == 0) paged_report(a.b.status, JV_ERR_RANGE, PS_ATTN_PAGE);
+            return -1;
+        }
+        return id;
+    };
+    int p0 = -1, p1 = -1, n0 = -1, n1 = -1;  // pages of the block whose K is next, and of the one after it
+    if (warp >= 8 && warp < 12) p0 = page_of(it.lo, 0), p1 = page_of(it.lo, 1), n0 = page_of(it.lo + 1, 0), n1 = page_of(it.lo + 1, 1);
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(k_full + 8 * i, 4);
@@ -245,19 +263,6 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
         reg_dec<128>();
         // ---------------------------------------------------- int8 -> fp16 operands
         const int t = tid - 256, j0 = t & 3, r0 = t >> 2;  // 16 bytes j0 and j0 + 4 of rows r0 + 32 k
-        const int32_t* table = a.b.block_table + (int64_t)item.x * a.b.max_blocks;
-        const int pages = (int)(((int64_t)it.rr.len + PG_TOKENS - 1) / PG_TOKENS);
-        // the two pages of a block; -1 where the request has none
-        auto page_of = [&](int b, int h) {
-            const int p = 2 * b + h;
-            if (b >= it.hi || p >= pages) return -1;
-            const int id = table[p];
-            if ((unsigned)id >= (unsigned)a.c.pages) {
-                if (t == 0) paged_report(err, JV_ERR_RANGE, PS_ATTN_PAGE);
-                return -1;
-            }
-            return id;
-        };
         uint4 kr[8], vr[8];
         auto load = [&](uint4 (&r)[8], int p0, int p1, int plane) {
 #pragma unroll
@@ -270,8 +275,6 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             }
         };
         // Block n's keys and scales; its bytes are in kr, its pages p0 and p1. Loads the next block's.
-        int p0 = page_of(it.lo, 0), p1 = page_of(it.lo, 1);        // of the block whose K is next
-        int n0 = page_of(it.lo + 1, 0), n1 = page_of(it.lo + 1, 1);  // and of the one after it
         auto keys = [&](int n) {
             const int b = it.lo + n;
             float4 sc = make_float4(0.f, 0.f, 1.f, 0.f);  // without a page nothing is visible
@@ -324,21 +327,37 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
         // ---------------------------------------------------- softmax and output, a query row per thread
         const int x = warp >> 2, r = tid & 127;
         const int b0 = it.b0[x], b1 = it.b1[x], nt = it.nt[x], t0 = it.t0[x];
-        const int tok = r / group, j = r - tok * group;
+        const uint32_t per_row = (65536u + group - 1) / group;  // row / group for rows below 128
+        auto token_of = [&](int row) { return (int)(((uint32_t)row * per_row) >> 16); };
+        const int tok = token_of(r);
         const bool live = tok < nt;
         const int pos = it.rr.len - it.rr.n_new + t0 + tok;
         // rows of no token see everything: they are not stored, and must not send their warp down the masked path
         const int hi_key = live ? pos + 1 : 1 << 30, lo_key = live && a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-        const int64_t token = it.rr.start + t0 + tok;
-        const int head = kvh * group + j;
+        const int64_t row0 = it.rr.start + t0;  // the tile's first token
+        uint8_t* tile = sm + x * KT_TILE;       // its queries, and at the end its output
         float qs = 0.f, qb = 0.f;
         if (b0 < b1) {
-            // the row to shared memory as fp16 (bf16: times a power of two, as in kv8_attn.cu), and its sum
+            // The row to shared memory as fp16 (bf16: times a power of two, as in kv8_attn.cu), and its sum. The loads take
+            // two rows at a time (a row per thread would touch 32 lines with each of them), so the rows go through
+            // shared memory on their way to their threads, too.
             uint32_t w[64];
 #pragma unroll
-            for (int c = 0; c < 16; c++) {
+            for (int i = 0; i < 16; i++) {
+                const int row = (warp & 3) * 32 + 2 * i + (lane >> 4), tk = token_of(row);
                 uint4 v = make_uint4(0, 0, 0, 0);
-                if (live) v = *(const uint4*)((const T*)a.q.in + token * a.q.in_token + (int64_t)head * a.q.in_head + 8 * c);
+                if (tk < nt)
+                    v = *(const uint4*)((const T*)a.q.in + (row0 + tk) * a.q.in_token + (int64_t)(kvh * group + row - tk * group) * a.q.in_head +
+                                        8 * (lane & 15));
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                *(uint4*)(tile + tile_off((warp & 3) * 32 + 2 * i + (lane >> 4), lane & 15)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 16; c++) {
+                const uint4 v = *(const uint4*)(tile + tile_off(r, c));
                 w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
             }
             float f = 1.f;
@@ -370,7 +389,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             qb = -128.f * sum * f;
 #pragma unroll
             for (int c = 0; c < 16; c++)
-                *(uint4*)(sm + x * KT_TILE + tile_off(r, c)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+                *(uint4*)(tile + tile_off(r, c)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full + 8 * x);
@@ -516,6 +535,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
             tc_fence_after();
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const int64_t part = ((int64_t)place * kvh_n + kvh) * 2 * PG_TILE + x * PG_TILE + r;
+            // the rows through shared memory (the queries' tile is free now), so that a store takes whole lines
 #pragma unroll 1
             for (int h = 0; h < 4; h++) {
                 uint32_t o[32];
@@ -526,9 +546,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
 #pragma unroll
                     for (int e = 0; e < 32; e++) o[e] = 0;
                 }
-                if (!live) continue;
                 if (splits == 1) {
-                    T* dst = (T*)a.q.out + token * a.q.out_token + (int64_t)head * a.q.out_head + 32 * h;
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
                         uint32_t y[4];
@@ -543,14 +561,30 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
                                 y[e] = *(const uint32_t*)&q;
                             }
                         }
-                        *(uint4*)(dst + 8 * c) = make_uint4(y[0], y[1], y[2], y[3]);
+                        *(uint4*)(tile + tile_off(r, 4 * h + c)) = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 } else if (any) {  // without a block, the reference of -infinity below says so
-                    float4* dst = (float4*)(a.large_o + part * PG_DIM + 32 * h);
 #pragma unroll
                     for (int c = 0; c < 8; c++)
-                        dst[c] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
-                                             __uint_as_float(o[4 * c + 3]));
+                        *(uint4*)(tile + tile_off(r, c)) = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int row = (warp & 3) * 32 + 4 * i + (lane >> 3);
+                        if (token_of(row) < nt)
+                            *(uint4*)(a.large_o + (part - r + row) * PG_DIM + 32 * h + 4 * (lane & 7)) = *(const uint4*)(tile + tile_off(row, lane & 7));
+                    }
+                    __syncwarp();
+                }
+            }
+            if (splits == 1) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int row = (warp & 3) * 32 + 2 * i + (lane >> 4), tk = token_of(row);
+                    if (tk < nt)
+                        *(uint4*)((T*)a.q.out + (row0 + tk) * a.q.out_token + (int64_t)(kvh * group + row - tk * group) * a.q.out_head + 8 * (lane & 15)) =
+                            *(const uint4*)(tile + tile_off(row, lane & 15));
                 }
             }
             if (live && splits > 1) a.large_ml[part] = make_float2(m, l);

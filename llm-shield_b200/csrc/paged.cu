@@ -104,6 +104,7 @@ PlanView plan_view(const jv_paged_batch& b) {
     v.prefix = (int32_t*)take(4 * R * 4);
     v.small_items = (int4*)take(v.small_cap * 32);
     v.large_items = (int4*)take(v.large_cap * 16);
+    v.large_rows = (int4*)take(v.large_cap * 16);
     v.units = (int4*)take(v.unit_cap * 16);
     v.bytes = at;
     return v;
@@ -173,8 +174,10 @@ __device__ __forceinline__ void plan_request(const PlanArgs& a, int r, const Pla
     const int large = large_of(q.old, q.n_new, b.group), pairs = pg_pairs(q.n_new, b.group);
     const int splits = large > 0 ? large / pairs : 1;
     // a request's last tiles see the most keys: first
-    for (int i = t; i < large; i += n)
+    for (int i = t; i < large; i += n) {
         a.v.large_items[q.large + i] = make_int4(r, pairs - 1 - i / splits, i % splits, splits | (splits > 1 ? (q.split + i) << 8 : 0));
+        a.v.large_rows[q.large + i] = make_int4(q.start, q.n_new, q.old + q.n_new, 0);
+    }
 }
 
 // One CTA: the sums over the requests and the checks; with `fill`, everything else too, a warp per

@@ -37,7 +37,7 @@ __host__ __device__ inline int pg_chunks(int len, int rows) {
 // Tokens of a large item (two tiles of 128 / group tokens), and the items of a request: its keys are split
 // too, in parts of at least 1024 keys, where it has at most 4 pairs of tiles: up to 16 items. (From 5 pairs on the
 // parts' results, 128 KB each, cost more than the balance gives: five chunks of 100 to 1500 tokens in a window
-// take 285 us without them, 317 with up to 16 items for up to 8 pairs, 461 with 32.) By the request's own sizes
+// took 285 us without them, 317 with up to 16 items for up to 8 pairs, 461 with 32.) By the request's own sizes
 // again.
 constexpr int PG_SPLIT_ITEMS = 16;  // a split of a pair is joined by a lane each
 __host__ __device__ inline int pg_pair_tokens(int group) { return 2 * (PG_TILE / group); }
@@ -55,6 +55,7 @@ struct PlanView {
     int32_t* prefix;    // [4][requests]: pages taken, units, large items and those with splits before request r
     int4* small_items;  // two each: {request, chunk, chunks, row tile}, {start, new, length, 0}; row tile by row tile
     int4* large_items;  // {request, pair of tiles, split, splits + 256 x place of its partials}; a pair's splits next to each other
+    int4* large_rows;   // beside each: {start, new, length, 0} of its request
     int4* units;        // the 16-token blocks the step writes to: {request, block, token of its row 0, first new row + 256 x end}
     int64_t small_cap, large_cap, split_cap, unit_cap, bytes;  // split_cap: most large items with more than one split
 };
