@@ -8,12 +8,13 @@
 //   w = 2^(e - M) as fp16 to shared memory (a row per thread, M moves only past 2^8)
 //   O += W V    (V MN-major)
 // TMEM: O_A, O_B, S_A, S_B, 128 columns each. A softmax hands its S columns back as soon as it has them in
-// registers, so the next block's S runs under its exponentials, and each tile has its own W: the softmaxes
-// never wait for the tensor pipe but at the start. (W over S in TMEM, which saves the shared memory, ran 213 to
-// 230 us where this took 195: S, softmax and W V one after the other.) A prompt of 4095 tokens, 32 / 8 heads: 182 us,
-// 752 TFLOP/s of visible work, about 4,700 cycles a block of the two tiles. What bounds it is the chain of the softmax
-// (scores out of TMEM, largest, exponentials, weights to shared memory) at two warps per scheduler: the exponential
-// unit is busy for 2,048 of them, the tensor pipe for 2,048, shared memory for about 3,200.
+// registers, so the next block's S runs under its exponentials, and each tile has its own W. (W over S in TMEM,
+// which saves the shared memory, ran 213 to 230 us where this took 195: S, softmax and W V one after the
+// other.) A prompt of 4095 tokens, 32 / 8 heads: 182 us, 752 TFLOP/s of visible work, about 4,700 cycles a
+// block of the two tiles, of which a softmax waits 950 for products. The exponential unit is busy for 2,048 of
+// them, the tensor pipe for 2,048 and shared memory, with 384 KB of operands, weights and converted keys and
+// values, for 3,072; with less work in the softmax a block took no fewer, so what is left is the products' way
+// through shared memory and the hand-overs around them.
 // Warps 0-3 and 4-7: the softmax and output of tiles A and B. Warps 8-11: convert the cache's int8 to fp16
 // operands (K as b + 128 in subnormals, one byte permute; V signed), two stages of K and one of V, in the
 // order K(b + 1), V(b), with the next blocks' bytes already in registers. Warps 12 and 13: issue tile A's and
