@@ -4,8 +4,9 @@
 // are the scales of key j's block of 16. The scales never touch the matrices: with
 //   e_j = scale ks(j) (q . kint_j) + log2 vs(j)   (in log2 units),   w_j = 2^(e_j - M),   M >= max e_j - 8
 // the output is  sum_j w_j vint_j / sum_j (w_j / vs(j)),  so the products run on exact integers (an
-// int8 is exact in fp16), w_j <= 2^8 is the only rounded operand (fp16, half a step 2^-11), and sums, M
-// and the softmax denominator are fp32. bf16 queries are taken to fp16 by a power of two per row.
+// int8 is exact in fp16), w_j <= 2^8 is the only rounded operand (fp16: half a step, 2^-11 of a weight above
+// 2^-14 and 2^-25 below), and sums, M and the softmax denominator are fp32. A block whose values are all zero
+// has vs = PG_ZERO_SCALE. bf16 queries are taken to fp16 by a power of two per row.
 //
 // Here: the requests of few query rows, whose time is the cache's bytes. (kv8_attn_tc.cu has the others.)
 // The products are mma.sync m16n8k16 with the keys on the 16-row side and the query rows (new token x
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(KS_WARPS * 32, Ks<NT>::ctas) k_kv8_small(AttnK
                 for (int h = 0; h < H; h++) {
                     ks_t[h] = ks[h];
                     // a block of zeros, or one without a key of the request
-                    vs_t[h] = vs[h] > 0.f && key0 + h * PG_BLOCK < cur.hi ? vs[h] : 1.f;
+                    vs_t[h] = vs[h] > 0.f && key0 + h * PG_BLOCK < cur.hi ? vs[h] : PG_ZERO_SCALE;
                 }
                 if ((t + 1) * KEYS < cur.hi) there = scales_of(cur, t + 1, ks, vs);
                 if (there_t) {

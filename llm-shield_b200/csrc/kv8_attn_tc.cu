@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
                 const int64_t key = (int64_t)b * KT_KEYS + t * PG_BLOCK;
                 if (id >= 0 && key < it.rr.len) {
                     const float* s = a.c.scales + (int64_t)id * a.c.scale_stride + kvh * 8 + (t & 3);
-                    const float vs = s[4] > 0.f ? s[4] : 1.f;  // a block of zeros
+                    const float vs = s[4] > 0.f ? s[4] : PG_ZERO_SCALE;
                     sc = make_float4(s[0], lg2_approx(vs), __frcp_rn(vs), 0.f);
                 }
             }

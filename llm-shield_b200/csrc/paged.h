@@ -34,6 +34,13 @@ __host__ __device__ inline int pg_chunks(int len, int rows) {
     return len <= 0 ? 0 : (int)(((int64_t)len + pg_chunk_keys(len, rows) - 1) / pg_chunk_keys(len, rows));
 }
 
+// The scale that a block of zero values (scale 0) counts as in attention. Its values are 0 at any scale, so only the
+// softmax's denominator takes it, in fp32; but log2 of it enters the exponents of which the largest is a row's
+// reference M, and a stand-in above the scales around it would push their fp16 weights down into subnormals (at 1,
+// values of 1e-4 beside zeros were 3 % off, and gone where the zeros' keys scored 2^8 above theirs). Below any
+// scale that values come with; not so far below that 2^-60 / (a large scale) would leave fp32.
+constexpr float PG_ZERO_SCALE = 0x1p-60f;
+
 // Tokens of a large item (two tiles of 128 / group tokens), and the items of a request: its keys are split
 // too, in parts of at least 1024 keys, where it has at most 4 pairs of tiles: up to 16 items. (From 5 pairs on the
 // parts' results, 128 KB each, cost more than the balance gives: five chunks of 100 to 1500 tokens in a window

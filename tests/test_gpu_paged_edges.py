@@ -1,0 +1,107 @@
+"""The paged-batch operators on the GPU where a result could depend on what it must not: the scales of blocks
+without values, the bounds of the batch, the alignment of an operand; and what is recorded when a result does not
+fit its type.
+
+Tolerance of the attention (`bounded`). A weight w_j = 2^(e_j - M), e_j = s_j + log2 vs_j, is rounded to fp16: by
+2^-11 of itself, or by 2^-25 where it is below 2^-14. The first adds up to 2^-11 sum p |v|. The second adds up to
+n 2^-25 127 / L with L = sum_j w_j / vs_j; since M is at most the row's largest e, that one's weight w_k is at least
+1, and 1 / L <= w_k / L = p_k vs_k, the largest of all p_j vs_j. fp32 arithmetic is taken as 2^-13 of sum p |v|
+(exponents below 2^7 carry an error of 2^-17 or less into a weight); the output is rounded to its type."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from test_gpu_paged import HALF, NUMERIC, RANGE, TYPE, Server, filled  # noqa: E402
+
+ZERO_SCALE = 2.0 ** -60  # what a block of zeros counts as
+
+
+def bounded(got, q, s, dtype, new, window=0, scale=128 ** -0.5):
+    """Every row of `got` against 64 bits; returns the largest error as a share of its bound."""
+    lengths, t, worst = s.lengths.tolist(), 0, 0.0
+    for r, n in enumerate(new):
+        if n == 0:
+            continue
+        kv = s.stored(r, lengths[r]).cuda()
+        pages = s.table[r, :-(-lengths[r] // 64)].long()
+        vs = s.scales.view(s.pages, s.scale_stride)[pages, :s.g * 8].view(-1, s.g, 2, 4)[:, :, 1].double()
+        vs = vs.permute(0, 2, 1).reshape(-1, s.g).repeat_interleave(16, 0)[:lengths[r]]
+        vs = torch.where(vs > 0, vs, ZERO_SCALE)
+        key = torch.arange(lengths[r], device="cuda")
+        at = torch.arange(lengths[r] - n, lengths[r], device="cuda")[:, None]
+        hide = key > at
+        if window:
+            hide |= key <= at - window
+        seen = (~hide).sum(-1)[:, None].double()
+        for h in range(s.g * s.group):
+            k, v = kv[0, :, h // s.group], kv[1, :, h // s.group]
+            p = torch.softmax((q[t:t + n, h].double() @ k.T * scale).masked_fill(hide, -math.inf), -1)
+            want, mag = p @ v, p @ v.abs()
+            low = seen * 2.0 ** -25 * 127 * (p * vs[:, h // s.group]).amax(-1, keepdim=True)
+            tol = HALF[dtype] * want.abs() + (2.0 ** -11 + 2.0 ** -13) * mag + low + (2.0 ** -25 if dtype == "f16" else 1e-38)
+            err = (got[t:t + n, h].double() - want).abs()
+            assert (err <= tol).all(), (r, h, float((err / tol).max()))
+            worst = max(worst, float((err / tol).max()))
+        t += n
+    return worst
+
+
+# (lengths before, new): one chunk, several chunks and their join, rows for the tensor cores, parts of a long
+# context and their join, both kinds in one call
+ROWS = [([40], [1]), ([700], [2]), ([90], [70]), ([3000], [40]), ([500, 1100], [1, 50])]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("amp", [0.1, 1e-3, 1e-4, 1e-6])
+@pytest.mark.parametrize("first,new", ROWS)
+def test_zero_values_among_small_ones(dtype, amp, first, new):
+    """One block of 16 values that are all zero, its keys some 8 log2 units above the others."""
+    g, group = 2, 4
+    requests, most = len(first), max(max(first), max(new))
+    blocks = -(-max(a + b for a, b in zip(first, new)) // 64)
+    s = Server(requests, g, group, requests * blocks, most, max(sum(first), sum(new)), blocks, seed=5)
+    gen = torch.Generator("cuda").manual_seed(11)
+    u = 128 ** -0.5 * torch.sign(torch.randn(128, generator=gen, device="cuda"))
+    for step in (first, new):
+        s.plan(step)
+        kv = torch.randn(sum(step), 2, g, 128, generator=gen, device="cuda")
+        kv[:, 1] *= amp
+        if step is first:
+            at = 0
+            for n in first:
+                kv[at + 16:at + 32, 1] = 0
+                kv[at + 16:at + 32, 0] += 8 * u  # q . k is 64 more, 8.2 in log2 units after the scale
+                at += n
+        s.append(kv[:, 0], kv[:, 1], "f32")
+    q = (torch.randn(sum(new), g * group, 128, generator=gen, device="cuda") + 8 * u).to(TYPE[dtype])
+    got = s.attend(q, dtype)
+    torch.cuda.synchronize()
+    assert s.status.tolist() == [0, 0]
+    bounded(got, q, s, dtype, new)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("first,new,window", [([400], [5], 40), ([300], [200], 32), ([1500], [60], 0), ([700, 90], [1, 33], 20)])
+def test_weights_carry_the_scales_of_their_blocks(dtype, first, new, window):
+    """Values from 1e-6 to 1e4 by block, some blocks zero; in a window a row may see zeros and tiny values alone."""
+    g, group = 2, 4
+    requests, most = len(first), max(max(first), max(new))
+    blocks = -(-max(a + b for a, b in zip(first, new)) // 64)
+    s = Server(requests, g, group, requests * blocks, most, max(sum(first), sum(new)), blocks, seed=6)
+    gen = torch.Generator("cuda").manual_seed(13)
+    for step in (first, new):
+        s.plan(step)
+        kv = torch.randn(sum(step), 2, g, 128, generator=gen, device="cuda")
+        mag = torch.tensor([1e-6, 0, 1e4, 1e-6, 0, 1e-3, 0, 1], device="cuda").repeat_interleave(16)
+        kv[:, 1] *= mag.repeat(-(-sum(step) // 128))[:sum(step), None, None]
+        s.append(kv[:, 0], kv[:, 1], "f32")
+    q = (2 * torch.randn(sum(new), g * group, 128, generator=gen, device="cuda")).to(TYPE[dtype])
+    got = s.attend(q, dtype, window=window)
+    torch.cuda.synchronize()
+    assert s.status.tolist() == [0, 0]
+    bounded(got, q, s, dtype, new, window)
