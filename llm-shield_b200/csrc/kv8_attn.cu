@@ -474,8 +474,11 @@ __global__ void __launch_bounds__(KS_WARPS * 32, Ks<NT>::ctas) k_kv8_small(AttnK
 }
 
 // Joins the chunks of small requests: one CTA per (row, request, KV head), its warps over the chunks with a
-// running reference each, four chunks' loads in flight. Latency-bound: 16 warps where a request can have more
-// than 128 chunks, else 4 (fewer idle warps per row).
+// running reference each, four chunks' loads in flight. Latency-bound: a request of more than KJ_FEW chunks takes 16
+// warps, the others 4. That goes by the request's own chunks, since the order of the sums, and with it the last
+// bits, goes by the warps; the batch's bounds only say how many the CTAs have (with 4 for tables of up to 512 pages,
+// which cannot hold more than KJ_FEW chunks, fewer warps are idle).
+constexpr int KJ_FEW = 128;
 template <class T, int KJ_WARPS>
 __global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
     __shared__ float4 so[KJ_WARPS][32];
@@ -489,16 +492,16 @@ __global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
     if (n_rows > PG_SMALL_ROWS || row >= n_rows || chunks < 2) return;
     const int item0 = first + row / PG_ROW_TILE * chunks;
     if (first < 0 || item0 + chunks > a.v.small_cap) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ways = chunks > KJ_FEW ? KJ_WARPS : 4;
     const int64_t p0 = ((int64_t)item0 * a.c.kv_heads + kvh) * a.rows + row % PG_ROW_TILE, step = (int64_t)a.c.kv_heads * a.rows;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float m = -INFINITY, l = 0.f;
-    for (int c0 = warp; c0 < chunks; c0 += 4 * KJ_WARPS) {
+    for (int c0 = warp < ways ? warp : chunks; c0 < chunks; c0 += 4 * ways) {
         float2 ml[4];
         float4 x[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const int c = c0 + k * KJ_WARPS;
+            const int c = c0 + k * ways;
             const bool in = c < chunks;
             ml[k] = in ? a.part_ml[p0 + c * step] : make_float2(-INFINITY, 0.f);
             x[k] = in ? *(const float4*)(a.part_o + (p0 + c * step) * PG_DIM + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -521,12 +524,14 @@ __global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
     if (warp) return;
     m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < KJ_WARPS; w++) m = fmaxf(m, sl[w].x);
+    for (int w = 0; w < KJ_WARPS; w++)
+        if (w < ways) m = fmaxf(m, sl[w].x);
     const float ref = m == -INFINITY ? 0.f : m;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
     l = 0.f;
 #pragma unroll
     for (int w = 0; w < KJ_WARPS; w++) {
+        if (w >= ways) break;
         const float f = ex2(sl[w].x - ref);
         const float4 x = so[w][lane];
         l = fmaf(sl[w].y, f, l);
@@ -608,7 +613,7 @@ void launch(const AttnKArgs& a, cudaStream_t s) {
         launch_small<T, 2>(a, ctas, s);
     if (a.b.max_keys > PG_CHUNK) {
         const dim3 grid(small_rows(a.b), a.b.requests, a.c.kv_heads);
-        if (a.b.max_blocks > 128 * 256 / PG_TOKENS)
+        if (a.b.max_blocks > KJ_FEW * 256 / PG_TOKENS)  // chunks of 256 keys and more
             launch_pdl(k_kv8_join<T, 16>, grid, dim3(16 * 32), 0, s, a);
         else
             launch_pdl(k_kv8_join<T, 4>, grid, dim3(4 * 32), 0, s, a);

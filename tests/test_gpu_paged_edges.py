@@ -105,3 +105,35 @@ def test_weights_carry_the_scales_of_their_blocks(dtype, first, new, window):
     torch.cuda.synchronize()
     assert s.status.tolist() == [0, 0]
     bounded(got, q, s, dtype, new, window)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("old,new,bounds", [
+    (300, 1, [(301, 6), (1, 6), (2000, 40), (1, 600), (2000, 600), (5, 513)]), (1500, 2, [(1502, 24), (2, 24), (2, 600), (3000, 513)]),
+    (2900, 5, [(2905, 46), (5, 46), (2905, 2000)]), (1300, 40, [(1340, 21), (40, 600)]),
+    (33000, 1, [(33001, 516), (1, 516), (1, 517), (40000, 3000)])])
+def test_a_request_s_bits_do_not_depend_on_the_batch_s_bounds(dtype, old, new, bounds):
+    """One request over the same cache, under other max_new and max_blocks."""
+    g, group, outs, data = 4, 4, [], None
+    gen = torch.Generator("cuda").manual_seed(old)
+    kv = torch.randn(old + new, 2, g, 128, generator=gen, device="cuda")
+    q = torch.randn(new, g * group, 128, generator=gen, device="cuda").to(TYPE[dtype])
+    held, pages = -(-old // 64), -(-(old + new) // 64)
+    for max_new, max_blocks in bounds:
+        s = Server(2, g, group, pages, max_new, max_new, max_blocks)
+        if data is None:  # the first one can take all tokens at once
+            s.plan([old + new, 0])
+            s.append(kv[:, 0], kv[:, 1], "f32")
+            data, scales, table = s.data.clone(), s.scales.clone(), s.table[0, :pages].clone()
+        s.data.copy_(data)
+        s.scales.copy_(scales)
+        s.table[0, :held] = table[:held]
+        s.free[:pages - held] = table[held:].flip(0)
+        s.n_free.fill_(pages - held)
+        s.lengths.copy_(torch.tensor([old, 0], dtype=torch.int32))
+        s.plan([new, 0])
+        outs.append(s.attend(q, dtype))
+        torch.cuda.synchronize()
+        assert s.status.tolist() == [0, 0] and s.lengths.tolist() == [old + new, 0]
+    for got in outs[1:]:
+        assert torch.equal(got.view(torch.int16), outs[0].view(torch.int16))
