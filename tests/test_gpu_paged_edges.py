@@ -86,7 +86,7 @@ def test_zero_values_among_small_ones(dtype, amp, first, new):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("first,new,window", [([400], [5], 40), ([300], [200], 32), ([1500], [60], 0), ([700, 90], [1, 33], 20)])
+@pytest.mark.parametrize("first,new,window", [([416], [5], 32), ([304], [200], 32), ([1504], [60], 0), ([704, 96], [1, 33], 20)])
 def test_weights_carry_the_scales_of_their_blocks(dtype, first, new, window):
     """Values from 1e-6 to 1e4 by block, some blocks zero; in a window a row may see zeros and tiny values alone."""
     g, group = 2, 4
