@@ -355,10 +355,9 @@ int jv_server_create(jv_model* model, int32_t max_requests, int32_t max_context,
 void jv_server_destroy(jv_server* server);
 /* One pass: request r brings counts[r] tokens (0: it sits the pass out), back to back in `tokens` in
  * request order. out[requests with tokens][n_rows] = logits of vocabulary `rows` at each one's last
- * token, in request order. JV_ERR_OOM when the pages run out and JV_ERR_RANGE when a request would
- * pass max_context leave every request as it was. An error found on the device (JV_ERR_NUMERIC) leaves
- * their lengths as they were; a block of 16 positions that the pass would have continued may have been
- * rounded once more. */
+ * token, in request order. A pass that fails leaves every request as it was: JV_ERR_OOM when the pages
+ * run out, JV_ERR_RANGE when a request would pass max_context, and errors found on the device
+ * (JV_ERR_NUMERIC; the blocks of 16 positions that the pass continued are put back). */
 int jv_server_forward(jv_server* server, const int32_t* tokens, const int32_t* counts, const int32_t* rows,
                       int32_t n_rows, float* out);
 /* Ends a request: its positions go to 0 and its pages back to the others. */

@@ -68,6 +68,20 @@ struct PlanView {
 };
 PlanView plan_view(const jv_paged_batch& b);
 
+// A page's planes of all layers, heads, K and V: plane p is int8 [64][128] at data + page * page_bytes + p * PG_PLANE,
+// its scales fp32 [4] at scales + page * scale_stride + 4 p.
+struct PagePlanes {
+    uint8_t* data;
+    float* scales;
+    int64_t page_bytes, scale_stride;
+    int pages, planes;
+};
+// Rows [y, y + z) of page x, less than a block of 16: the tokens of a request in the block that its next token
+// continues. An append to the block may round them again, so who must be able to take a step back copies them (and
+// the block's scale) to `saved`, n * planes * PG_SAVED bytes, and from there.
+constexpr int PG_SAVED = PG_BLOCK * PG_DIM + 16;
+void launch_kv8_save_blocks(const PagePlanes& c, const int4* blocks, int n, uint8_t* saved, bool restore, cudaStream_t s);
+
 void check_batch(const jv_paged_batch* b, bool arrays);
 void check_cache(const jv_kv8_cache* c);
 void check_rows(const jv_heads* x, const char* name, int dim, int64_t tokens);

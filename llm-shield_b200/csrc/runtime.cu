@@ -1422,6 +1422,7 @@ struct jv_server {
     std::vector<jv_kv8_cache> layers;
     int64_t page_bytes = 0, scale_stride = 0, ws_bytes = 0;
     DevVec<uint8_t> data, work, ws;
+    DevVec<uint8_t> saved;  // of the pass under way: the blocks that it continues, as they were
     DevVec<float> scales;
     DevVec<int32_t> d_table, d_lengths, d_starts, d_request, d_positions, d_free, d_counts, d_status;  // counts: new, n_free
     DevVec<int64_t> d_slots;
@@ -1462,6 +1463,7 @@ void server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, 
         if (len > v->max_context)
             throw Error(JV_ERR_RANGE, "request " + std::to_string(r) + " would pass its " + std::to_string(v->max_context) + " positions");
         need += (len + PG_TOKENS - 1) / PG_TOKENS - (int64_t)v->table[r].size();
+        v->table[r].reserve((size_t)((len + PG_TOKENS - 1) / PG_TOKENS));  // nothing can fail after the pass has gone through
         T += counts[r];
         if (counts[r] > 0) outputs.push_back((int32_t)(T - 1));
     }
@@ -1484,9 +1486,20 @@ void server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, 
     cudaStream_t s = x->stream;
     if (v->dirty) server_upload(v);  // and nothing of a failed pass is under way any more
     // one upload: tokens, outputs, rows, counts
-    const size_t words = (size_t)n + n_out + n_rows + v->max_requests;
+    // (in front of them, for their alignment: the blocks of 16 positions that the pass continues)
+    std::vector<int32_t> open;
+    for (int r = 0; r < v->max_requests; r++)
+        if (counts[r] > 0 && v->lengths[r] % PG_BLOCK != 0)
+            open.insert(open.end(), {v->table[r].back(), v->lengths[r] % PG_TOKENS / PG_BLOCK * PG_BLOCK, v->lengths[r] % PG_BLOCK, 0});
+    const int n_open = (int)open.size() / 4;
+    const PagePlanes planes = {v->data.p, v->scales.p, v->page_bytes, v->scale_stride, v->pages, c.layers * c.kv_heads * 2};
+    const size_t words = open.size() + n + n_out + n_rows + v->max_requests;
     int32_t* hin = x->h_in.get(words);
-    int32_t* din = x->in_i32.get(words);
+    int32_t* const up = x->in_i32.get(words);
+    int32_t* const din = up + open.size();
+    std::copy(open.begin(), open.end(), hin);
+    const int32_t* const h_up = hin;
+    hin += open.size();
     std::memcpy(hin, tokens, 4 * (size_t)n);
     std::memcpy(hin + n, outputs.data(), 4 * (size_t)n_out);
     std::memcpy(hin + n + n_out, rows, 4 * (size_t)n_rows);
@@ -1500,7 +1513,26 @@ void server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, 
     __half* ctx16 = x->ctx16.get((size_t)tpad * qdim);
     __half* xf = x->xs_ff.get((size_t)tpad * ff);
     v->dirty = true;  // until the pass has gone through
-    JV_CUDA(cudaMemcpyAsync(din, hin, 4 * words, cudaMemcpyHostToDevice, s));
+    JV_CUDA(cudaMemcpyAsync(up, h_up, 4 * words, cudaMemcpyHostToDevice, s));
+    // An append rounds the entries of a block that it continues again when the block's scale grows. A pass that fails
+    // on the way must not leave them so: their requests go on without its tokens.
+    struct Undo {
+        jv_server* v;
+        const PagePlanes& planes;
+        const int4* open;
+        int n;
+        ~Undo() {
+            if (n == 0) return;
+            try {
+                launch_kv8_save_blocks(planes, open, n, v->saved.p, true, v->x->stream);
+            } catch (...) {  // a device that takes no launch takes no further pass either
+            }
+        }
+    } undo{v, planes, (const int4*)up, 0};
+    if (n_open > 0) {
+        launch_kv8_save_blocks(planes, undo.open, n_open, v->saved.p, false, s);
+        undo.n = n_open;
+    }
     rc_check(jv_paged_plan(&v->batch, v->d_lengths.p, din + n + n_out + n_rows, v->d_free.p, v->d_counts.p + v->max_requests,
                            v->d_counts.p + v->max_requests, s));
     launch_embed(m->embd, din, n, h, hidden, x->d_err, s);
@@ -1549,6 +1581,7 @@ void server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, 
             v->free_pages.pop_back();
         }
     }
+    undo.n = 0;
     v->dirty = false;
     if (n_rows > 0) std::memcpy(out, hres, sizeof(float) * n_out * n_rows);
     x->resolve_profile();
@@ -1991,6 +2024,9 @@ int jv_server_create(jv_model* m, int32_t max_requests, int32_t max_context, int
         v->ws.get((size_t)v->ws_bytes);
         uint8_t* data = v->data.get((size_t)v->pages * v->page_bytes);
         float* scales = v->scales.get((size_t)v->pages * v->scale_stride);
+        // a request of the pass brings a token, and holds a page
+        const int64_t most = std::min<int64_t>(std::min(max_requests, max_tokens), v->pages);
+        v->saved.get((size_t)(most * c.layers * c.kv_heads * 2 * PG_SAVED));
         v->free_pages.resize(v->pages);
         for (int i = 0; i < v->pages; i++) v->free_pages[i] = v->pages - 1 - i;
         for (int l = 0; l < c.layers; l++)
@@ -2010,7 +2046,7 @@ void jv_server_destroy(jv_server* v) {
     if (!v) return;
     cudaSetDevice(v->m->device);
     if (v->x) cudaStreamSynchronize(v->x->stream);
-    for (auto* d : {&v->data, &v->work, &v->ws}) d->release();
+    for (auto* d : {&v->data, &v->work, &v->ws, &v->saved}) d->release();
     for (auto* d : {&v->d_table, &v->d_lengths, &v->d_starts, &v->d_request, &v->d_positions, &v->d_free, &v->d_counts, &v->d_status})
         d->release();
     v->scales.release();
