@@ -94,7 +94,9 @@ __device__ __forceinline__ void store_row(const AttnKArgs& a, int start, int kvh
     const float inv = l == 0.f ? 0.f : 1.f / l;  // no visible key: zeros (a NaN stays one)
     T* dst = (T*)a.q.out + (int64_t)(start + row / a.b.group) * a.q.out_token +
              (int64_t)(kvh * a.b.group + row % a.b.group) * a.q.out_head + 4 * d4;
-    *(uint2*)dst = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+    o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+    if (outside<T>(o)) paged_report(a.b.status, JV_ERR_NUMERIC, PS_ATTN_VALUE);
+    *(uint2*)dst = make_uint2(pack2<T>(o.x, o.y), pack2<T>(o.z, o.w));
 }
 
 // ------------------------------------------------------------ small requests

@@ -535,6 +535,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
         } else {
             tc_fence_after();
             const float inv = l == 0.f ? 0.f : 1.f / l;
+            __half2 most = __floats2half2_rn(0.f, 0.f);  // the row's largest fp16 outputs: infinities and NaN stay
             const int64_t part = ((int64_t)place * kvh_n + kvh) * 2 * PG_TILE + x * PG_TILE + r;
             // the rows through shared memory (the queries' tile is free now), so that a store takes whole lines
 #pragma unroll 1
@@ -556,6 +557,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
                             const float y0 = __uint_as_float(o[8 * c + 2 * e]) * inv, y1 = __uint_as_float(o[8 * c + 2 * e + 1]) * inv;
                             if (std::is_same<T, __half>::value) {
                                 const __half2 q = __floats2half2_rn(y0, y1);
+                                most = __hmax2_nan(most, __habs2(q));
                                 y[e] = *(const uint32_t*)&q;
                             } else {
                                 const __nv_bfloat162 q = __floats2bfloat162_rn(y0, y1);
@@ -588,6 +590,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
                             *(const uint4*)(tile + tile_off(row, lane & 15));
                 }
             }
+            if (live && !(__half2float(__hmax_nan(__low2half(most), __high2half(most))) < 65520.f)) paged_report(err, JV_ERR_NUMERIC, PS_ATTN_VALUE);
             if (live && splits > 1) a.large_ml[part] = make_float2(m, l);
         }
     }
@@ -603,13 +606,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
 // take a row each.
 constexpr int KTJ_WARPS = 8;
 template <class T>
-__device__ __forceinline__ void join_row(const AttnKArgs& a, int4 item, int kvh, int row, int lane) {
+__device__ __forceinline__ bool join_row(const AttnKArgs& a, int4 item, int kvh, int row, int lane) {
     const int splits = item.w & 255, place = item.w >> 8;
     RequestRows rr;
-    if (splits > PG_SPLIT_ITEMS || place < 0 || place + splits > a.v.split_cap || !request_rows(a.b, item.x, rr)) return;
+    if (splits > PG_SPLIT_ITEMS || place < 0 || place + splits > a.v.split_cap || !request_rows(a.b, item.x, rr)) return false;
     const int group = a.b.group, tt = PG_TILE / group, x = row / PG_TILE, r = row % PG_TILE, tok = r / group;
     const int t = item.y * 2 * tt + x * tt + tok;
-    if (tok >= tt || t < 0 || t >= rr.n_new) return;
+    if (tok >= tt || t < 0 || t >= rr.n_new) return false;
     const int64_t p0 = ((int64_t)place * a.c.kv_heads + kvh) * 2 * PG_TILE + row, step = (int64_t)a.c.kv_heads * 2 * PG_TILE;
     const float2 ml = lane < splits ? a.large_ml[p0 + lane * step] : make_float2(-INFINITY, 0.f);  // at most 16 splits
     float m = ml.x;
@@ -629,17 +632,20 @@ __device__ __forceinline__ void join_row(const AttnKArgs& a, int4 item, int kvh,
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* dst = (T*)a.q.out + (int64_t)(rr.start + t) * a.q.out_token + (int64_t)(kvh * group + r - tok * group) * a.q.out_head + 4 * lane;
+    o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
     if (std::is_same<T, __half>::value) {
-        const __half2 u = __floats2half2_rn(o.x * inv, o.y * inv), v = __floats2half2_rn(o.z * inv, o.w * inv);
+        const __half2 u = __floats2half2_rn(o.x, o.y), v = __floats2half2_rn(o.z, o.w);
         *(uint2*)dst = make_uint2(*(const uint32_t*)&u, *(const uint32_t*)&v);
     } else {
-        const __nv_bfloat162 u = __floats2bfloat162_rn(o.x * inv, o.y * inv), v = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+        const __nv_bfloat162 u = __floats2bfloat162_rn(o.x, o.y), v = __floats2bfloat162_rn(o.z, o.w);
         *(uint2*)dst = make_uint2(*(const uint32_t*)&u, *(const uint32_t*)&v);
     }
+    return outside<T>(o);
 }
 template <class T>
 __global__ void __launch_bounds__(KTJ_WARPS * 32) k_kv8_large_join(AttnKArgs a) {
     pdl_wait();
+    bool out_of_range = false;
     const int lane = threadIdx.x & 31, warp = blockIdx.x * KTJ_WARPS + (threadIdx.x >> 5), warps = gridDim.x * KTJ_WARPS;
     const int n = (int)min((int64_t)a.v.head[1], a.v.large_cap);
     for (int i0 = 0; i0 < n; i0 += 32) {
@@ -649,9 +655,11 @@ __global__ void __launch_bounds__(KTJ_WARPS * 32) k_kv8_large_join(AttnKArgs a) 
             const int src = __ffs(some) - 1;
             const int4 item = make_int4(__shfl_sync(0xffffffffu, mine.x, src), __shfl_sync(0xffffffffu, mine.y, src),
                                         __shfl_sync(0xffffffffu, mine.z, src), __shfl_sync(0xffffffffu, mine.w, src));
-            for (int u = warp; u < a.c.kv_heads * 2 * PG_TILE; u += warps) join_row<T>(a, item, u / (2 * PG_TILE), u % (2 * PG_TILE), lane);
+            for (int u = warp; u < a.c.kv_heads * 2 * PG_TILE; u += warps)
+                out_of_range |= join_row<T>(a, item, u / (2 * PG_TILE), u % (2 * PG_TILE), lane);
         }
     }
+    if (out_of_range) paged_report(a.b.status, JV_ERR_NUMERIC, PS_ATTN_VALUE);
 }
 
 template <class T>

@@ -2,6 +2,8 @@
 // layout of the 8-bit cache and of a plan's work lists, and the host-side checks.
 #pragma once
 
+#include <type_traits>
+
 #include "jv_internal.h"
 
 namespace jv {
@@ -113,7 +115,7 @@ int paged_api(F&& f) {
 enum PagedSite : int {
     PS_PLAN_LENGTH = 96, PS_PLAN_TOKENS = 97, PS_PLAN_KEYS = 98, PS_PLAN_FREE = 99, PS_PLAN_PAGE = 100,
     PS_APPEND_PAGE = 101, PS_APPEND_VALUE = 102, PS_READ_SLOT = 103, PS_READ_VALUE = 104,
-    PS_ATTN_PAGE = 106, PS_ROPE_VALUE = 107, PS_ATTN_WAIT = 108, PS_ATTN_TC = 112 /* + role */
+    PS_ATTN_VALUE = 105, PS_ATTN_PAGE = 106, PS_ROPE_VALUE = 107, PS_ATTN_WAIT = 108, PS_ATTN_TC = 112 /* + role */
 };
 
 // An attention launch.
@@ -137,6 +139,13 @@ void launch_kv8_large(const AttnKArgs& a, int type, cudaStream_t s);
 __device__ __forceinline__ void paged_report(int32_t* status, int code, int site) {
     if (!status) return;
     if (atomicCAS(status, 0, code) == 0) atomicExch(status + 1, site);
+}
+
+// Outputs about to be rounded to T: whether one becomes an fp16 infinity or is not a number.
+template <class T>
+__device__ __forceinline__ bool outside(float4 o) {
+    return std::is_same<T, __half>::value &&
+           (f16_out_of_range(o.x) || f16_out_of_range(o.y) || f16_out_of_range(o.z) || f16_out_of_range(o.w));
 }
 
 // The request's rows of a plan, as an operator after it uses them; false (and a report) where the

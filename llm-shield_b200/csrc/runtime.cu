@@ -1570,7 +1570,7 @@ void server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, 
     sync_check(x);
     if (status[0] != 0)
         throw Error(status[0], status[0] == JV_ERR_NUMERIC
-                                   ? "a rotated query, or a key or value for the 8-bit cache, is not in the fp16 range or not a number"
+                                   ? "a rotated query or an attention output is outside the fp16 range, or a key or value for the 8-bit cache is not finite"
                                : status[0] == JV_ERR_DEVICE_TIMEOUT ? "a device-side wait timed out (attention over the 8-bit cache)"
                                                                     : "a paged-batch operator refused the pass (site " + std::to_string(status[1]) + ")");
     // the pass went through: the device's lengths, tables and free list are the host's

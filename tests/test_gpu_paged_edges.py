@@ -137,3 +137,18 @@ def test_a_request_s_bits_do_not_depend_on_the_batch_s_bounds(dtype, old, new, b
         assert s.status.tolist() == [0, 0] and s.lengths.tolist() == [old + new, 0]
     for got in outs[1:]:
         assert torch.equal(got.view(torch.int16), outs[0].view(torch.int16))
+
+
+@pytest.mark.parametrize("first,new", ROWS)
+def test_an_output_outside_fp16_is_recorded(first, new):
+    """Values of 1e5 as fp16 outputs: infinities, and JV_ERR_NUMERIC; as bf16 outputs neither."""
+    s, _ = filled(len(new), 2, 4, first, new, "f16", 7)
+    s.scales *= 1e5  # keys too: a row picks one of them
+    q = 1e-4 * torch.randn(sum(new), 8, 128, device="cuda")
+    got = s.attend(q.bfloat16(), "bf16")
+    torch.cuda.synchronize()
+    assert s.status.tolist() == [0, 0] and torch.isfinite(got).all()
+    assert got.abs().max() > 65520
+    got = s.attend(q.half(), "f16")
+    torch.cuda.synchronize()
+    assert not torch.isfinite(got).all() and s.status.tolist() == [NUMERIC, 105]
