@@ -89,14 +89,15 @@ __device__ __forceinline__ float q_to_f16(uint32_t (&q)[16]) {
     return up;
 }
 
+// Stores four outputs of a row; true where fp16 does not hold one.
 template <class T>
-__device__ __forceinline__ void store_row(const AttnKArgs& a, int start, int kvh, int row, int d4, float4 o, float l) {
+__device__ __forceinline__ bool store_row(const AttnKArgs& a, int start, int kvh, int row, int d4, float4 o, float l) {
     const float inv = l == 0.f ? 0.f : 1.f / l;  // no visible key: zeros (a NaN stays one)
     T* dst = (T*)a.q.out + (int64_t)(start + row / a.b.group) * a.q.out_token +
              (int64_t)(kvh * a.b.group + row % a.b.group) * a.q.out_head + 4 * d4;
     o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
-    if (outside<T>(o)) paged_report(a.b.status, JV_ERR_NUMERIC, PS_ATTN_VALUE);
     *(uint2*)dst = make_uint2(pack2<T>(o.x, o.y), pack2<T>(o.z, o.w));
+    return outside<T>(o);
 }
 
 // ------------------------------------------------------------ small requests
@@ -442,6 +443,7 @@ __global__ void __launch_bounds__(KS_WARPS * 32, Ks<NT>::ctas) k_kv8_small(AttnK
                 else
                     flight--;
             }
+            bool out_of_range = false;
             // the chunk's result: lane (g, i) holds dimensions 16 g .. + 15 of rows 2 i and 2 i + 1
 #pragma unroll
             for (int n = 0; n < NT; n++)
@@ -456,8 +458,8 @@ __global__ void __launch_bounds__(KS_WARPS * 32, Ks<NT>::ctas) k_kv8_small(AttnK
                     if (cur.chunks == 1) {
 #pragma unroll
                         for (int j = 0; j < 8; j += 2)
-                            store_row<T>(a, cur.start, cur.kvh, cur.row0 + row, 4 * g + j / 2,
-                                         make_float4(acc[n][j][c], acc[n][j][c + 2], acc[n][j + 1][c], acc[n][j + 1][c + 2]), x);
+                            out_of_range |= store_row<T>(a, cur.start, cur.kvh, cur.row0 + row, 4 * g + j / 2,
+                                                         make_float4(acc[n][j][c], acc[n][j][c + 2], acc[n][j + 1][c], acc[n][j + 1][c + 2]), x);
                     } else {
                         const int64_t p = ((int64_t)cur.item * kvh_n + cur.kvh) * a.rows + row;
                         float4* dst = (float4*)(a.part_o + p * PG_DIM + 16 * g);
@@ -467,6 +469,7 @@ __global__ void __launch_bounds__(KS_WARPS * 32, Ks<NT>::ctas) k_kv8_small(AttnK
                         if (g == 0) a.part_ml[p] = make_float2(m[n][c], x);
                     }
                 }
+            if (out_of_range) paged_report(a.b.status, JV_ERR_NUMERIC, PS_ATTN_VALUE);
         }
         // what the next item still lacks of its first stages (all of them after an item without keys)
         cur = nxt;
@@ -481,29 +484,20 @@ __global__ void __launch_bounds__(KS_WARPS * 32, Ks<NT>::ctas) k_kv8_small(AttnK
 // bits, goes by the warps; the batch's bounds only say how many the CTAs have (with 4 for tables of up to 512 pages,
 // which cannot hold more than KJ_FEW chunks, fewer warps are idle).
 constexpr int KJ_FEW = 128;
-template <class T, int KJ_WARPS>
-__global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
-    __shared__ float4 so[KJ_WARPS][32];
-    __shared__ float2 sl[KJ_WARPS];
-    pdl_wait();
-    const int row = blockIdx.x, request = blockIdx.y, kvh = blockIdx.z;
-    RequestRows rr;
-    const int first = a.v.first[request];  // asked for together with the rows
-    if (!request_rows(a.b, request, rr)) return;
-    const int n_rows = rr.n_new * a.b.group, chunks = pg_chunks(rr.len, n_rows);
-    if (n_rows > PG_SMALL_ROWS || row >= n_rows || chunks < 2) return;
-    const int item0 = first + row / PG_ROW_TILE * chunks;
-    if (first < 0 || item0 + chunks > a.v.small_cap) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ways = chunks > KJ_FEW ? KJ_WARPS : 4;
-    const int64_t p0 = ((int64_t)item0 * a.c.kv_heads + kvh) * a.rows + row % PG_ROW_TILE, step = (int64_t)a.c.kv_heads * a.rows;
+// The row's chunks by WAYS warps.
+template <class T, int WAYS>
+__device__ __forceinline__ void join_chunks(const AttnKArgs& a, const RequestRows& rr, int row, int kvh, int chunks, int64_t p0,
+                                            float4 (*so)[32], float2* sl) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t step = (int64_t)a.c.kv_heads * a.rows;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float m = -INFINITY, l = 0.f;
-    for (int c0 = warp < ways ? warp : chunks; c0 < chunks; c0 += 4 * ways) {
+    for (int c0 = warp < WAYS ? warp : chunks; c0 < chunks; c0 += 4 * WAYS) {
         float2 ml[4];
         float4 x[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const int c = c0 + k * ways;
+            const int c = c0 + k * WAYS;
             const bool in = c < chunks;
             ml[k] = in ? a.part_ml[p0 + c * step] : make_float2(-INFINITY, 0.f);
             x[k] = in ? *(const float4*)(a.part_o + (p0 + c * step) * PG_DIM + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -520,26 +514,45 @@ __global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
             o.x = fmaf(x[k].x, f, o.x), o.y = fmaf(x[k].y, f, o.y), o.z = fmaf(x[k].z, f, o.z), o.w = fmaf(x[k].w, f, o.w);
         }
     }
-    so[warp][lane] = o;
-    if (lane == 0) sl[warp] = make_float2(m, l);
+    if (warp < WAYS) {
+        so[warp][lane] = o;
+        if (lane == 0) sl[warp] = make_float2(m, l);
+    }
     __syncthreads();
     if (warp) return;
     m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < KJ_WARPS; w++)
-        if (w < ways) m = fmaxf(m, sl[w].x);
+    for (int w = 0; w < WAYS; w++) m = fmaxf(m, sl[w].x);
     const float ref = m == -INFINITY ? 0.f : m;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
     l = 0.f;
 #pragma unroll
-    for (int w = 0; w < KJ_WARPS; w++) {
-        if (w >= ways) break;
+    for (int w = 0; w < WAYS; w++) {
         const float f = ex2(sl[w].x - ref);
         const float4 x = so[w][lane];
         l = fmaf(sl[w].y, f, l);
         o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
     }
-    store_row<T>(a, rr.start, kvh, row, lane, o, l);
+    if (store_row<T>(a, rr.start, kvh, row, lane, o, l)) paged_report(a.b.status, JV_ERR_NUMERIC, PS_ATTN_VALUE);
+}
+template <class T, int KJ_WARPS>
+__global__ void __launch_bounds__(KJ_WARPS * 32) k_kv8_join(AttnKArgs a) {
+    __shared__ float4 so[KJ_WARPS][32];
+    __shared__ float2 sl[KJ_WARPS];
+    pdl_wait();
+    const int row = blockIdx.x, request = blockIdx.y, kvh = blockIdx.z;
+    RequestRows rr;
+    const int first = a.v.first[request];  // asked for together with the rows
+    if (!request_rows(a.b, request, rr)) return;
+    const int n_rows = rr.n_new * a.b.group, chunks = pg_chunks(rr.len, n_rows);
+    if (n_rows > PG_SMALL_ROWS || row >= n_rows || chunks < 2) return;
+    const int item0 = first + row / PG_ROW_TILE * chunks;
+    if (first < 0 || item0 + chunks > a.v.small_cap) return;
+    const int64_t p0 = ((int64_t)item0 * a.c.kv_heads + kvh) * a.rows + row % PG_ROW_TILE;
+    if (KJ_WARPS > 4 && chunks > KJ_FEW)
+        join_chunks<T, KJ_WARPS>(a, rr, row, kvh, chunks, p0, so, sl);
+    else
+        join_chunks<T, 4>(a, rr, row, kvh, chunks, p0, so, sl);
 }
 
 // Query rows of a small item, and row tiles of a small request, at most.
