@@ -335,7 +335,7 @@ int64_t jv_kv8_attention_bytes(const jv_paged_batch* batch, int32_t kv_heads);
 /* Grouped-query attention of the batch's new tokens over the cache (their own keys appended before):
  * q->in, [tokens][kv_heads * group][128] of `type` (F16 or BF16), to q->out of the same type. The token
  * at position p sees keys p - window + 1 .. p, or 0 .. p when window is 0. A token without a visible key
- * gives zeros. An F16 output outside the type's range becomes an infinity; that, and an F16 output that is not
+ * gives zeros; the keys of a page that is not in the cache (recorded as JV_ERR_RANGE) have no weight. An F16 output outside the type's range becomes an infinity; that, and an F16 output that is not
  * a number, is recorded as JV_ERR_NUMERIC. The result of a request depends on its own tokens only, bit for bit,
  * not on what else is in the batch. Rows of q start on 16 bytes. */
 int jv_kv8_attention(const jv_kv8_cache* cache, const jv_paged_batch* batch, int32_t type, const jv_heads* q, float scale,

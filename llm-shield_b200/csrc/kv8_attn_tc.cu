@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_large(AttnKArgs a) {
         // Block n's keys and scales; its bytes are in kr, its pages p0 and p1. Loads the next block's.
         auto keys = [&](int n) {
             const int b = it.lo + n;
-            float4 sc = make_float4(0.f, 0.f, 1.f, 0.f);  // without a page nothing is visible
+            float4 sc = make_float4(0.f, -INFINITY, 1.f, 0.f);  // keys without a page have no weight
             if (t < 8) {
                 const int id = t < 4 ? p0 : p1;
                 const int64_t key = (int64_t)b * KT_KEYS + t * PG_BLOCK;

@@ -152,3 +152,23 @@ def test_an_output_outside_fp16_is_recorded(first, new):
     got = s.attend(q.half(), "f16")
     torch.cuda.synchronize()
     assert not torch.isfinite(got).all() and s.status.tolist() == [NUMERIC, 105]
+
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 1], [70, 90]])
+def test_keys_of_a_bad_page_have_no_weight(new):
+    """A request whose first page is not in the cache: the result of its other keys."""
+    s, q = filled(2, 1, 4, [200, 100], new, "f16", 8)
+    torch.cuda.synchronize()
+    assert s.status.tolist() == [0, 0]
+    s.table[0, 0] = s.pages
+    got = s.attend(q, "f16")
+    torch.cuda.synchronize()
+    assert s.status.tolist() == [RANGE, 106]
+    s.table[0, 0] = 0
+    kv = s.stored(0, 200 + new[0])[:, 64:, 0]
+    for i in range(new[0]):
+        x = kv[:, :200 + i + 1 - 64]
+        p = torch.softmax(q[i].double().cpu() @ x[0].T * 128 ** -0.5, -1)
+        mag = p @ x[1].abs()
+        tol = HALF["f16"] * (p @ x[1]).abs() + (2.0 ** -11 + 2.0 ** -13) * mag + 300 * 2.0 ** -25 * x[1].abs().max() + 2.0 ** -25
+        assert ((got[i].double().cpu() - p @ x[1]).abs() <= tol).all()
