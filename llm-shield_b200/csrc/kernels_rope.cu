@@ -143,8 +143,8 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope(RopeKArgs a, int per_cta) {
         float u = ld1(in + e0), v = ld1(in + e1);
         if (p < half) {
             const float2 c = cs[t][p];
-            const float r = __fsub_rn(__fmul_rn(u, c.x), __fmul_rn(v, c.y));
-            v = __fadd_rn(__fmul_rn(u, c.y), __fmul_rn(v, c.x));
+            const float r = fmaf(-v, c.y, u * c.x);  // as rotate_vec has it: alignment changes no bits
+            v = fmaf(u, c.y, v * c.x);
             u = r;
         }
         st1(out + e0, u * k);

@@ -172,3 +172,22 @@ def test_keys_of_a_bad_page_have_no_weight(new):
         mag = p @ x[1].abs()
         tol = HALF["f16"] * (p @ x[1]).abs() + (2.0 ** -11 + 2.0 ** -13) * mag + 300 * 2.0 ** -25 * x[1].abs().max() + 2.0 ** -25
         assert ((got[i].double().cpu() - p @ x[1]).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("layout,rot,dim", [("interleaved", 128, 128), ("half", 128, 128), ("half", 64, 128), ("interleaved", 96, 128)])
+def test_rope_s_bits_do_not_depend_on_the_alignment(dtype, layout, rot, dim):
+    from jevstral_b200 import paged
+
+    spec = paged.rope_spec(layout, rot, 1e4, temperature_scale=0.1, temperature_context=64)
+    x = torch.randn(300, 5, dim, generator=torch.Generator("cuda").manual_seed(rot), device="cuda").to(TYPE[dtype])
+    pos = torch.arange(1000, 1300, dtype=torch.int32, device="cuda")
+    outs = []
+    for offset in (0, 1):
+        src = torch.zeros(x.numel() + 8, device="cuda", dtype=x.dtype)[offset:offset + x.numel()].view_as(x)
+        src.copy_(x)
+        out = torch.empty_like(x)
+        paged.rope(spec, dtype, pos.data_ptr(), 300, dim, paged.heads(src.data_ptr(), 5, 5 * dim, dim, out.data_ptr(), temperature=True))
+        outs.append(out)
+    torch.cuda.synchronize()
+    assert torch.equal(*outs)
