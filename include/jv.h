@@ -259,7 +259,8 @@ typedef struct jv_paged_batch {
     int32_t* status;      /* [2]                                                           */
 } jv_paged_batch;
 
-/* Bytes of jv_paged_batch.work for the batch's bounds; -1 and jv_last_error on a bad one. */
+/* Bytes of jv_paged_batch.work for the batch's bounds; -1 and jv_last_error on a bad one, or where they allow
+ * 2^30 chunks of work (64 to 2048 keys of 16 query rows) or more, which every operator refuses. */
 int64_t jv_paged_work_bytes(const jv_paged_batch* batch);
 
 /* Block tables and slot maps from the requests' lengths. Request r holds cached[r] tokens, whose

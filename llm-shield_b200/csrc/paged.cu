@@ -29,6 +29,8 @@ void check_batch(const jv_paged_batch* b, bool arrays) {
          "max_keys must be at most requests * max_blocks * 64");
     need(b->group >= 1 && b->group <= PG_MAX_GROUP, "group must be 1 to 16 query heads per KV head");
     need(b->pages >= 1, "the cache needs at least one page");
+    // a small item is two entries of its list, which the plan indexes in 32 bits
+    need(plan_view(*b).small_cap < (1 << 30), "the batch's bounds allow 2^30 work items or more");
     if (!arrays) return;
     need(b->block_table && b->lengths && b->starts && b->request_of && b->positions && b->slots && b->work && b->status,
          "a batch array is NULL");
