@@ -674,6 +674,8 @@ int jv_kv8_attention(const jv_kv8_cache* cache, const jv_paged_batch* batch, int
         const Workspace w = workspace(*batch, cache->kv_heads);
         if (workspace_bytes < w.bytes) throw Error(JV_ERR_ARG, "attention: the workspace is smaller than jv_kv8_attention_bytes");
         if (!ws || (uintptr_t)ws % 16) throw Error(JV_ERR_ARG, "attention: the workspace must be 16-byte aligned");
+        if (plan_view(*batch).large_cap > INT32_MAX / cache->kv_heads)
+            throw Error(JV_ERR_RANGE, "attention: too many tokens and KV heads for one call");
         OnDeviceOf dev(cache->data);
         AttnKArgs a{};
         a.c = *cache;

@@ -676,8 +676,7 @@ void launch_large(const AttnKArgs& a, cudaStream_t s) {
         if (at.numRegs != 128) throw Error(JV_ERR_DEVICE, "k_kv8_large was not built with 128 registers per thread");
         done.fetch_or(bit);
     }
-    if (a.v.large_cap > INT32_MAX / a.c.kv_heads) throw Error(JV_ERR_RANGE, "attention: too many tokens and KV heads for one call");
-    const unsigned items = (unsigned)(a.v.large_cap * a.c.kv_heads);
+    const unsigned items = (unsigned)(a.v.large_cap * a.c.kv_heads);  // jv_kv8_attention has seen that it fits
     launch_pdl(k_kv8_large<T>, dim3(items), dim3(KT_THREADS), KT_SMEM, s, a);
     note_launch();
     if (a.v.split_cap > 0 && a.b.max_blocks > 16) {  // a request of at most 1024 keys has no splits

@@ -16,3 +16,14 @@ def test_a_batch_whose_work_lists_would_pass_32_bits_is_refused():
     assert lib.jv_paged_plan(C.byref(b), 64, 64, 64, 64, 64, None) == JV_ERR_ARG
     b.max_keys = 4096 * 262144  # the same requests of 262,144 keys
     assert lib.jv_paged_work_bytes(C.byref(b)) > 0
+
+
+def test_attention_refuses_too_many_items_before_it_queues_any():
+    """2^24 pairs of query tiles and 1024 KV heads pass a grid's 2^31 blocks: refused by the host, ahead of the first
+    launch (a call that got that far would fail for want of a device here)."""
+    from jevstral_b200._lib import JV_ERR_RANGE, lib
+
+    b = _batch(requests=1, max_new=1 << 28, max_tokens=1 << 28, max_blocks=1 << 22, max_keys=1 << 28, group=16)
+    c = _cache(kv_heads=1024, page_bytes=1024 * 16384, scale_stride=1024 * 8)
+    q = _heads(16384)
+    assert lib.jv_kv8_attention(C.byref(c), C.byref(b), 1, C.byref(q), 0.1, 0, 64, 1 << 62, None) == JV_ERR_RANGE
