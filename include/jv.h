@@ -317,9 +317,10 @@ int jv_rope(const jv_rope_spec* spec, int32_t type, const int32_t* positions, in
  * bits. A block of 16 tokens has one scale per head for K and one for V: the largest magnitude written
  * to it / 127. Where a block holds tokens of earlier steps the scale grows if it must, and their entries
  * are rounded again at the new scale. With `rope` the keys are rotated first (rotary_dim a multiple of 8,
- * at most 128) and, with q, the queries too: q->in of `type` to q->out of out_type. A value that is not
- * finite is recorded as JV_ERR_NUMERIC; it is stored as 0 (not a number) or the block's largest value
- * (an infinity) and does not count for the scale. Magnitudes below 2^-100 are stored as 0. */
+ * at most 128) and, with q, the queries too: q->in of `type` to q->out of out_type. Only q may ask for the
+ * query temperature. A value that is not finite is recorded as JV_ERR_NUMERIC; it is stored as 0 (not a
+ * number) or the block's largest value (an infinity) and does not count for the scale. Magnitudes below
+ * 2^-100 are stored as 0. */
 int jv_kv8_append(const jv_kv8_cache* cache, const jv_paged_batch* batch, int32_t type, const jv_heads* k,
                   const jv_heads* v, const jv_rope_spec* rope, const jv_heads* q, int32_t out_type, void* stream);
 

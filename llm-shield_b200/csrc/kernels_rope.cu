@@ -682,6 +682,7 @@ int jv_kv8_append(const jv_kv8_cache* cache, const jv_paged_batch* batch, int32_
         if (elem == 0) throw Error(JV_ERR_UNSUPPORTED, "the type must be F32 (0), F16 (1) or BF16 (30)");
         check_heads(k, "k", cache->kv_heads, elem, true, false);
         check_heads(v, "v", cache->kv_heads, elem, true, false);
+        if (k->temperature || v->temperature) throw Error(JV_ERR_ARG, "the query temperature is for q, not for k or v");
         AppendArgs a{};
         a.c = *cache;
         a.b = *batch;

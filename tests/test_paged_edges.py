@@ -27,3 +27,14 @@ def test_attention_refuses_too_many_items_before_it_queues_any():
     c = _cache(kv_heads=1024, page_bytes=1024 * 16384, scale_stride=1024 * 8)
     q = _heads(16384)
     assert lib.jv_kv8_attention(C.byref(c), C.byref(b), 1, C.byref(q), 0.1, 0, 64, 1 << 62, None) == JV_ERR_RANGE
+
+
+def test_append_refuses_the_query_temperature_on_keys_and_values():
+    """The flag is the queries': keys or values that ask for it would not get it."""
+    from jevstral_b200._lib import JV_ERR_ARG, JvRopeSpec, lib
+
+    spec = JvRopeSpec()
+    assert lib.jv_rope_init(C.byref(spec), 0, 64, 1e4, 0, 1, 0, 32, 1, 1) == 0
+    b, c, plain, hot = _batch(), _cache(), _heads(2), _heads(2, temperature=1)
+    for k, v in ((hot, plain), (plain, hot)):
+        assert lib.jv_kv8_append(C.byref(c), C.byref(b), 1, C.byref(k), C.byref(v), C.byref(spec), None, 1, None) == JV_ERR_ARG
