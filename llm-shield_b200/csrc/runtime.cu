@@ -1478,7 +1478,6 @@ void server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, 
     for (int i = 0; i < n_rows; i++)
         if ((unsigned)rows[i] >= (unsigned)m->head.rows)
             throw Error(JV_ERR_RANGE, "vocabulary row " + std::to_string(rows[i]) + " is out of range");
-    check_cancel(x);
 
     const int n = (int)T, n_out = (int)outputs.size();
     const int hidden = c.hidden, qdim = c.heads * c.head_dim, kvdim = c.kv_heads * c.head_dim, qkvn = qdim + 2 * kvdim, ff = c.ff;
@@ -1538,7 +1537,6 @@ void server_forward(jv_server* v, const int32_t* tokens, const int32_t* counts, 
     launch_embed(m->embd, din, n, h, hidden, x->d_err, s);
     const float* resid = nullptr;
     for (int l = 0; l < c.layers; l++) {
-        check_cancel(x);
         const LayerW& W = m->layers[l];
         launch_rmsnorm_resid(h, resid, W.attn_norm, n, hidden, c.eps, xs, tpad, x->d_err, s);
         gemm(x, W.qkv, xs, n, tpad, qkv, qkvn, EPI_STORE);
