@@ -536,7 +536,7 @@ bool vec4(const void* p, int64_t a, int64_t b, int elem) {
 
 template <class T>
 void launch_rope(const RopeKArgs& a, int n, cudaStream_t s) {
-    const int tiles = (a.tokens + RP_TOKENS - 1) / RP_TOKENS;
+    const int tiles = (a.tokens - 1) / RP_TOKENS + 1;  // tokens is 1 to 2^31 - 1
     // enough CTAs for the SMs when the tokens are few: the heads are split
     const int split = std::max(1, std::min(a.n_heads, 1184 / std::max(1, tiles)));
     const int per = (a.n_heads + split - 1) / split;

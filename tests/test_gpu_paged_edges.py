@@ -191,3 +191,21 @@ def test_rope_s_bits_do_not_depend_on_the_alignment(dtype, layout, rot, dim):
         outs.append(out)
     torch.cuda.synchronize()
     assert torch.equal(*outs)
+
+
+def test_rope_of_the_most_tokens():
+    """2^31 - 1 tokens of one pair each, in place: the first, the last and some between (17 GB)."""
+    from jevstral_b200 import paged
+
+    n = 2 ** 31 - 1
+    spec = paged.rope_spec("interleaved", 2, 1e4)
+    x = torch.ones(n, 2, dtype=torch.float16, device="cuda")
+    pos = torch.full((n,), 7, dtype=torch.int32, device="cuda")
+    at = torch.tensor([0, 1, 12345678, 2 ** 30 + 3, n - 8, n - 2, n - 1], device="cuda")
+    pos[at] = torch.arange(1, len(at) + 1, dtype=torch.int32, device="cuda")
+    paged.rope(spec, "f16", pos.data_ptr(), n, 2, paged.heads(x.data_ptr(), 1, 2, 2, x.data_ptr()))
+    torch.cuda.synchronize()
+    angle = pos[at].double()
+    want = torch.stack([angle.cos() - angle.sin(), angle.cos() + angle.sin()], 1)
+    # cos and sin to 3 units of 2^-23, their sum of at most 1.42; then half a step of fp16
+    assert ((x[at].double() - want).abs() <= HALF["f16"] * want.abs() + 8 * 2.0 ** -23).all()
