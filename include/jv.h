@@ -337,9 +337,14 @@ int64_t jv_kv8_attention_bytes(const jv_paged_batch* batch, int32_t kv_heads);
 /* Grouped-query attention of the batch's new tokens over the cache (their own keys appended before):
  * q->in, [tokens][kv_heads * group][128] of `type` (F16 or BF16), to q->out of the same type. The token
  * at position p sees keys p - window + 1 .. p, or 0 .. p when window is 0. A token without a visible key
- * gives zeros; the keys of a page that is not in the cache (recorded as JV_ERR_RANGE) have no weight. An F16 output outside the type's range becomes an infinity; that, and an F16 output that is not
- * a number, is recorded as JV_ERR_NUMERIC. The result of a request depends on its own tokens only, bit for bit,
- * not on what else is in the batch. Rows of q start on 16 bytes. */
+ * gives zeros; the keys of a page that is not in the cache (recorded as JV_ERR_RANGE) have no weight. An
+ * F16 output outside the type's range becomes an infinity; that, and an F16 output that is not a number, is
+ * recorded as JV_ERR_NUMERIC. The result of a request depends on its own tokens only, bit for bit, not on
+ * what else is in the batch or on its bounds. Rows of q start on 16 bytes.
+ * Scores, exponents, sums and the softmax's denominator are fp32; a weight is rounded to fp16 before it meets
+ * the values, by half a step (2^-11 of itself, or 2^-25 of the row's largest product of weight and block scale
+ * where that is more). That holds for values of 2^-50 to 2^40 where blocks of zeros are beside them, and for
+ * |scale * q| up to 2^110. */
 int jv_kv8_attention(const jv_kv8_cache* cache, const jv_paged_batch* batch, int32_t type, const jv_heads* q, float scale,
                      int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -8,9 +8,10 @@
 //   w = 2^(e - M) as fp16 to shared memory (a row per thread, M moves only past 2^8)
 //   O += W V    (V MN-major)
 // TMEM: O_A, O_B, S_A, S_B, 128 columns each. A softmax hands its S columns back as soon as it has them in
-// registers, so the next block's S runs under its exponentials, and each tile has its own W. (W over S in TMEM,
-// which saves the shared memory, ran 213 to 230 us where this took 195: S, softmax and W V one after the
-// other.) A prompt of 4095 tokens, 32 / 8 heads: 182 us, 752 TFLOP/s of visible work, about 4,700 cycles a
+// registers, so the next block's S runs under its exponentials, and each tile has its own W. (W over S in TMEM
+// would save a third of the shared-memory traffic. It was measured before the packed arithmetic, the register split
+// and the halves below: 230 us, 213 with the tiles taking turns, where W in shared memory took 219 at that
+// point; not since.) A prompt of 4095 tokens, 32 / 8 heads: 183 us, 750 TFLOP/s of visible work, about 4,700 cycles a
 // block of the two tiles, of which a softmax waits 950 for products. The exponential unit is busy for 2,048 of
 // them, the tensor pipe for 2,048 and shared memory, with 384 KB of operands, weights and converted keys and
 // values, for 3,072; with less work in the softmax a block took no fewer, so what is left is the products' way

@@ -39,15 +39,16 @@ __host__ __device__ inline int pg_chunks(int len, int rows) {
 // The scale that a block of zero values (scale 0) counts as in attention. Its values are 0 at any scale, so only the
 // softmax's denominator takes it, in fp32; but log2 of it enters the exponents of which the largest is a row's
 // reference M, and a stand-in above the scales around it would push their fp16 weights down into subnormals (at 1,
-// values of 1e-4 beside zeros were 3 % off, and gone where the zeros' keys scored 2^8 above theirs). Below any
-// scale that values come with; not so far below that 2^-60 / (a large scale) would leave fp32.
+// values of 1e-4 beside zeros were 3 % off, and gone where the zeros' keys scored 2^8 above theirs). So it is below any
+// scale that values of 2^-50 or more come with, and beside values up to 2^40 weights down to 2^-32 of the largest are still an fp32.
 constexpr float PG_ZERO_SCALE = 0x1p-60f;
 
 // Tokens of a large item (two tiles of 128 / group tokens), and the items of a request: its keys are split
-// too, in parts of at least 1024 keys, where it has at most 4 pairs of tiles: up to 16 items. (From 5 pairs on the
-// parts' results, 128 KB each, cost more than the balance gives: five chunks of 100 to 1500 tokens in a window
-// took 285 us without them, 317 with up to 16 items for up to 8 pairs, 461 with 32.) By the request's own sizes
-// again.
+// too, in parts of at least 1024 keys, where it has at most 4 pairs of tiles: up to 16 items. By the request's own
+// sizes again. The parts go by the whole length, also in a window, where most of them then have no block: the end at
+// 4 pairs was measured there (five chunks of 100 to 1500 tokens in a window of 4096: 285 us, 317 with up to 16 items
+// for up to 8 pairs, 461 with 32). For a lone request without a window it is a cliff: 256 tokens on 30,000 keys
+// take 173 us, 257 tokens 543.
 constexpr int PG_SPLIT_ITEMS = 16;  // a split of a pair is joined by a lane each
 __host__ __device__ inline int pg_pair_tokens(int group) { return 2 * (PG_TILE / group); }
 __host__ __device__ inline int pg_pairs(int n_new, int group) { return (n_new + pg_pair_tokens(group) - 1) / pg_pair_tokens(group); }
