@@ -357,7 +357,9 @@ int jv_kv8_attention(const jv_kv8_cache* cache, const jv_paged_batch* batch, int
  * the pass. */
 
 /* max_context: most positions of a request; max_tokens: most new tokens of one pass; pages: pages of
- * 64 positions shared by the requests (0 = max_context positions for every request). */
+ * 64 positions shared by the requests (0 = max_context positions for every request). Beside the pages the
+ * server holds a quarter of a page for each request that a pass can continue (at most max_requests,
+ * max_tokens and pages), to put back what a failed pass changed. */
 int jv_server_create(jv_model* model, int32_t max_requests, int32_t max_context, int32_t max_tokens, int32_t pages,
                      jv_server** out);
 void jv_server_destroy(jv_server* server);
